@@ -42,6 +42,7 @@ enum zgpu_dtype {
    * path: dequant.rs:63-138, 286-356): 144 / 210 bytes per super-block. */
   ZGPU_Q4_K = 12,
   ZGPU_Q6_K = 14,
+  ZGPU_BF16 = 30, /* rows given to the paged 4-bit cache */
   ZGPU_Q4_0X4 = 100,
   ZGPU_Q8_0X4 = 101
 };
@@ -262,6 +263,109 @@ zgpu_status zgpu_gqa_attention_decode_noalloc(zgpu_ctx *ctx, zgpu_kv *kv, uint32
                                               const float *d_q_norm, const float *d_k_norm,
                                               const float *d_inv_freqs, float eps, float *d_out,
                                               void *stream);
+
+/* ------------------------------------------------ paged 4-bit KV cache */
+/* Has no counterpart in the reference, whose cache is one f32 array per
+ * sequence (kv_cache.rs:32): a pool of blocks that many sequences share, with
+ * keys and values held in 4 bits, 144 bytes per token, layer and kv head
+ * instead of 1024.
+ *
+ * Format.  A token's K or V row of one head is four groups of 32 values; a
+ * group is one scale d and integers q in -8..7 and stands for q * d.  With m
+ * the group's value of largest magnitude (the first of equals), d is -m / 8
+ * rounded to 8 significant bits and then to binary16, and q the integer
+ * nearest to x / d, ties to even, clamped to -8..7.  A group with a
+ * non-finite value, or one of a magnitude above 21760, is stored as zeros and
+ * recorded as ZGPU_ERR_NUMERICAL_INSTABILITY.
+ *
+ * Slots.  A pool has n_blocks blocks of block_tokens token slots; slot
+ * number = block * block_tokens + offset, ZGPU_KV4_NONE for none.  A block
+ * table row lists a sequence's blocks in order.  Lengths, tables, slots and
+ * row starts are arrays of uint32_t in device memory, so that a step's sizes
+ * need not be known to the host.
+ *
+ * Calls.  The _device entry points launch on `stream` (NULL: the context's
+ * stream; cudaStreamLegacy names the default stream) without synchronising,
+ * allocating or changing the caller's current device, and may be captured.
+ * Rows start on 16-byte boundaries, and strides (elements between tokens, 0:
+ * dense) are multiples of 16 bytes, so k, v and q may be columns of a fused
+ * projection's rows.  dtype is ZGPU_F32, ZGPU_F16 or ZGPU_BF16.  Errors found
+ * on the device are kept with the cache until zgpu_kv4_check reads them; no
+ * bad slot, block or length leads outside the buffers.  Calls on one cache
+ * that write what another reads have to be ordered by the caller, as on one
+ * stream. */
+typedef struct zgpu_kv4 zgpu_kv4;
+typedef struct zgpu_kv4_work zgpu_kv4_work;
+#define ZGPU_KV4_NONE 0xFFFFFFFFu
+/* A zeroed pool.  block_tokens is 16, 32, 64 or 128, head_dim 128, and the
+ * pool has fewer than 2^31 slots. */
+zgpu_status zgpu_kv4_create(zgpu_ctx *ctx, uint32_t n_blocks, uint32_t block_tokens, uint32_t n_layers,
+                            uint32_t n_kv_heads, uint32_t head_dim, zgpu_kv4 **out);
+void zgpu_kv4_destroy(zgpu_kv4 *kv);
+/* Scratch of the attention: one serves one call at a time.  Calls that may
+ * overlap on the GPU (two streams, two graphs replayed side by side) need one
+ * each. */
+zgpu_status zgpu_kv4_work_create(zgpu_ctx *ctx, zgpu_kv4_work **out);
+void zgpu_kv4_work_destroy(zgpu_kv4_work *work);
+/* Waits for the context's stream, then reports and clears the first of the
+ * errors that device calls recorded: ZGPU_ERR_KV_TOKEN_OUT_OF_RANGE (a slot,
+ * block or length outside the cache), ZGPU_ERR_KV_TOKEN_COUNT_EXCEEDS_MAX (a
+ * refused plan or release), ZGPU_ERR_NUMERICAL_INSTABILITY.  A caller that
+ * used other streams waits for them first. */
+zgpu_status zgpu_kv4_check(zgpu_kv4 *kv);
+/* Plans one step of n_seq (1..1024) rows: row i holds d_old_lens[i] tokens and
+ * gets d_new_lens[i] (0 allowed) more.  Blocks come from the end of
+ * d_free_list [n_blocks], whose first d_state_in[0] entries are free, in row
+ * order.  Writes the table (rows of table_width blocks, ZGPU_KV4_NONE behind
+ * the last), d_slots [n_slots] (the new tokens' slots, row after row, then
+ * ZGPU_KV4_NONE), d_starts [n_seq + 1] (the rows' first tokens), d_kv_lens
+ * [n_seq] (old + new) and d_state_out [4]: free blocks left, 0, new tokens,
+ * blocks taken.  A step that does not fit takes nothing: d_state_out[1] is 1
+ * (too few free blocks) or 2 (a row beyond its table, more tokens than
+ * n_slots), the table keeps its blocks, every slot is ZGPU_KV4_NONE, every
+ * start 0 and every length the old one.  d_table_out may be d_table_in; no
+ * other output may overlap an input. */
+zgpu_status zgpu_kv4_plan_device(zgpu_kv4 *kv, uint32_t n_seq, uint32_t table_width, const uint32_t *d_old_lens,
+                                 const uint32_t *d_new_lens, const uint32_t *d_table_in, uint32_t *d_table_out,
+                                 const uint32_t *d_free_list, const uint32_t *d_state_in, uint32_t *d_state_out,
+                                 uint32_t n_slots, uint32_t *d_slots, uint32_t *d_starts, uint32_t *d_kv_lens,
+                                 void *stream);
+/* Returns the blocks of the rows with d_done[i] != 0 to the free list, in row
+ * order: their lengths become 0, their table entries ZGPU_KV4_NONE,
+ * d_state[0] grows, d_state[1..3] become 0, 0 and the blocks returned.  A
+ * table with a block outside the pool, or more blocks than the pool has,
+ * changes nothing but d_state[1] = 2. */
+zgpu_status zgpu_kv4_release_device(zgpu_kv4 *kv, uint32_t n_seq, uint32_t table_width, const uint32_t *d_done,
+                                    uint32_t *d_lens, uint32_t *d_table, uint32_t *d_free_list, uint32_t *d_state,
+                                    void *stream);
+/* Quantises k and v rows [n_tokens][n_kv_heads * 128] into the slots of
+ * d_slots [n_tokens]; a token with ZGPU_KV4_NONE is skipped.  No slot may be
+ * named twice in one call. */
+zgpu_status zgpu_kv4_append_device(zgpu_kv4 *kv, uint32_t layer, uint32_t n_tokens, const void *d_k, uint64_t k_stride,
+                                   const void *d_v, uint64_t v_stride, uint32_t dtype, const uint32_t *d_slots,
+                                   void *stream);
+/* The values that the slots stand for, as rows (zeros for ZGPU_KV4_NONE);
+ * d_k or d_v may be NULL.  f32 and f16 hold them exactly. */
+zgpu_status zgpu_kv4_gather_device(zgpu_kv4 *kv, uint32_t layer, uint32_t n_tokens, const uint32_t *d_slots, void *d_k,
+                                   uint64_t k_stride, void *d_v, uint64_t v_stride, uint32_t dtype, void *stream);
+/* Causal attention of a ragged batch over the cache: query rows
+ * [n_rows][n_q_heads * 128] (normed and rotated), those of sequence i at
+ * d_starts[i] .. d_starts[i + 1] - 1, being the last of its d_kv_lens[i]
+ * cached tokens: query t of n sees keys 0 .. d_kv_lens[i] - n + t.
+ * out = softmax(scale * q k^T) v in the same layout and type; a query that
+ * sees no key gets zeros, and rows behind the last sequence's are left as
+ * they are.  n_q_heads is 1..16 x n_kv_heads, head h reading kv head
+ * h / (n_q_heads / n_kv_heads); max_q is at least every sequence's number of
+ * queries.  Sums and softmax are held in f32; with ZGPU_F32 rows the products
+ * keep 22 bits of q and of the probabilities, with 16-bit rows at least
+ * binary16's 11.  out must not overlap q.  A sequence with more than max_q
+ * queries, or whose rows are not within n_rows, gets no output; keys whose
+ * block is not in the pool are left out; both are recorded. */
+zgpu_status zgpu_kv4_attention_device(zgpu_kv4 *kv, zgpu_kv4_work *work, uint32_t layer, uint32_t n_seq,
+                                      uint32_t n_rows, uint32_t max_q, uint32_t n_q_heads, const void *d_q,
+                                      uint64_t q_stride, void *d_out, uint64_t out_stride, uint32_t dtype,
+                                      const uint32_t *d_starts, const uint32_t *d_kv_lens, const uint32_t *d_table,
+                                      uint32_t table_width, float scale, void *stream);
 
 /* ------------------------------------------------------------ Qwen3 model */
 /* One decoder layer's tensors, each a registered host key (LayerWeights,

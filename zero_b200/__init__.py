@@ -20,6 +20,8 @@ from .synth import DS2_V2_LITE, QWEN3_1_7B, Ds2Config, Qwen3Config
 
 ABI_VERSION = 1
 F32, F16, Q4_0, Q8_0, Q4_0X4, Q8_0X4 = 0, 1, 2, 8, 100, 101
+BF16 = 30               # rows given to the paged 4-bit cache
+KV4_NONE = 0xFFFFFFFF   # ZGPU_KV4_NONE: no slot, no block
 Q4_K, Q6_K = 12, 14     # GGUF K-quants (plain rows of 256-element super-blocks)
 IPC_HANDLE_BYTES = 64   # ZGPU_IPC_HANDLE_BYTES
 FLAG_NO_GRAPH, FLAG_NO_PDL, FLAG_NO_PERSISTENT = 0x1, 0x2, 0x4
@@ -260,6 +262,100 @@ class KvCache:
         self.ctx._check(LIB.zgpu_gqa_attention_decode(self.ctx.h, self.h, layer, pos, n_q_heads, _ptr(qkv),
                                                       _ptr(qn), _ptr(kn), freq_base, eps, _ptr(out)))
         return out
+
+
+class KvCache4:
+    """A paged KV cache in 4 bits (zgpu_kv4_*): a pool of blocks for many
+    sequences, with the step plan, the append and the attention that go with it.
+
+    The ``*_device`` methods take device addresses (``tensor.data_ptr()``) of
+    caller-owned memory and a stream handle (0: the context's stream, 1: the
+    legacy default stream) and do not synchronise.  ``check()`` raises what
+    earlier calls recorded on the device.  The attention uses the cache's own
+    workspace unless it is given another (``new_work``): calls that may overlap
+    on the GPU need one each."""
+
+    def __init__(self, ctx: Context, n_blocks: int, block_tokens: int, n_layers: int, n_kv_heads: int,
+                 head_dim: int = 128):
+        self.h = self.work = None
+        self.ctx = ctx
+        self.n_blocks, self.block_tokens, self.n_layers = n_blocks, block_tokens, n_layers
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+        h = C.c_void_p()
+        ctx._check(LIB.zgpu_kv4_create(ctx.h, n_blocks, block_tokens, n_layers, n_kv_heads, head_dim, C.byref(h)))
+        self.h = h
+        self.work = KvCache4Work(ctx)
+
+    def close(self):
+        if self.h:
+            LIB.zgpu_kv4_destroy(self.h)
+            self.h = None
+        if self.work:
+            self.work.close()
+
+    def __del__(self):
+        self.close()
+
+    def new_work(self) -> "KvCache4Work":
+        return KvCache4Work(self.ctx)
+
+    def check(self):
+        self.ctx._check(LIB.zgpu_kv4_check(self.h))
+
+    def plan_device(self, n_seq: int, table_width: int, d_old_lens: int, d_new_lens: int, d_table_in: int,
+                    d_table_out: int, d_free_list: int, d_state_in: int, d_state_out: int, n_slots: int, d_slots: int,
+                    d_starts: int, d_kv_lens: int, stream: int = 0):
+        """Block table, slots, row starts and lengths of one step (zgpu_kv4_plan_device)."""
+        self.ctx._check(LIB.zgpu_kv4_plan_device(self.h, n_seq, table_width, d_old_lens, d_new_lens, d_table_in,
+                                                 d_table_out, d_free_list, d_state_in, d_state_out, n_slots, d_slots,
+                                                 d_starts, d_kv_lens, stream or None))
+
+    def release_device(self, n_seq: int, table_width: int, d_done: int, d_lens: int, d_table: int, d_free_list: int,
+                       d_state: int, stream: int = 0):
+        """Blocks of the rows marked done go back to the free list (zgpu_kv4_release_device)."""
+        self.ctx._check(LIB.zgpu_kv4_release_device(self.h, n_seq, table_width, d_done, d_lens, d_table, d_free_list,
+                                                    d_state, stream or None))
+
+    def append_device(self, layer: int, n_tokens: int, d_k: int, d_v: int, d_slots: int, dtype: int = F32,
+                      k_stride: int = 0, v_stride: int = 0, stream: int = 0):
+        """Rows k, v into slots, quantised (zgpu_kv4_append_device)."""
+        self.ctx._check(LIB.zgpu_kv4_append_device(self.h, layer, n_tokens, d_k, k_stride, d_v, v_stride, dtype,
+                                                   d_slots, stream or None))
+
+    def gather_device(self, layer: int, n_tokens: int, d_slots: int, d_k: int, d_v: int, dtype: int = F32,
+                      k_stride: int = 0, v_stride: int = 0, stream: int = 0):
+        """The values of slots as rows (zgpu_kv4_gather_device)."""
+        self.ctx._check(LIB.zgpu_kv4_gather_device(self.h, layer, n_tokens, d_slots, d_k, k_stride, d_v, v_stride,
+                                                   dtype, stream or None))
+
+    def attention_device(self, layer: int, n_seq: int, n_rows: int, max_q: int, n_q_heads: int, d_q: int, d_out: int,
+                         d_starts: int, d_kv_lens: int, d_table: int, table_width: int, dtype: int = F32,
+                         scale: float | None = None, q_stride: int = 0, out_stride: int = 0, stream: int = 0,
+                         work: "KvCache4Work | None" = None):
+        """Causal attention of a ragged batch over the cache (zgpu_kv4_attention_device)."""
+        self.ctx._check(LIB.zgpu_kv4_attention_device(
+            self.h, (work or self.work).h, layer, n_seq, n_rows, max_q, n_q_heads, d_q, q_stride, d_out, out_stride,
+            dtype, d_starts, d_kv_lens, d_table, table_width, self.head_dim ** -0.5 if scale is None else scale,
+            stream or None))
+
+
+class KvCache4Work:
+    """Scratch of KvCache4.attention_device (zgpu_kv4_work_create): one per
+    call that may be on the GPU at a time."""
+
+    def __init__(self, ctx: Context):
+        self.h = None
+        h = C.c_void_p()
+        ctx._check(LIB.zgpu_kv4_work_create(ctx.h, C.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h:
+            LIB.zgpu_kv4_work_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
 
 
 class Qwen3Model:

@@ -172,6 +172,17 @@ _SIGS = {
     "zgpu_ds2_decode_batch": (_i32, [_vp, _vp, _u32, _vp, _vp, _vp, _vp]),
     "zgpu_ds2_batch_expert_ids": (_i32, [_vp, _u32, _vp, _vp]),
     "zgpu_ds2_perf_snapshot": (_i32, [_vp, C.POINTER(ZgpuPerf)]),
+    "zgpu_kv4_create": (_i32, [_vp, _u32, _u32, _u32, _u32, _u32, C.POINTER(_vp)]),
+    "zgpu_kv4_destroy": (None, [_vp]),
+    "zgpu_kv4_work_create": (_i32, [_vp, C.POINTER(_vp)]),
+    "zgpu_kv4_work_destroy": (None, [_vp]),
+    "zgpu_kv4_check": (_i32, [_vp]),
+    "zgpu_kv4_plan_device": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
+    "zgpu_kv4_release_device": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "zgpu_kv4_append_device": (_i32, [_vp, _u32, _u32, _vp, _u64, _vp, _u64, _u32, _vp, _vp]),
+    "zgpu_kv4_gather_device": (_i32, [_vp, _u32, _u32, _vp, _vp, _u64, _vp, _u64, _u32, _vp]),
+    "zgpu_kv4_attention_device": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _vp, _u64, _u32, _vp, _vp,
+                                         _vp, _u32, _f, _vp]),
     "zgpu_synth_q4_0": (None, [_u64, _u64, _u64, _u64, _f, _vp]),
     "zgpu_synth_q8_0": (None, [_u64, _u64, _u64, _u64, _f, _vp]),
     "zgpu_synth_f32": (None, [_u64, _u64, _u64, _f, _f, _vp]),

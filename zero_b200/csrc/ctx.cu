@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "digit_mma.h"
 #include "internal.h"
+#include "kv4.h"
 #include "layout.h"
 #include "ops.h"
 #include "step.h"
@@ -96,6 +97,7 @@ zgpu_status zgpu_init(const zgpu_opts *opts, zgpu_ctx **out) {
       zgpu::ops_setup() != cudaSuccess || zgpu::step_setup() != cudaSuccess ||
       zgpu::moe_setup() != cudaSuccess || zgpu::mla_setup() != cudaSuccess ||
       zgpu::prefill_setup() != cudaSuccess || zgpu::mma_setup() != cudaSuccess || zgpu::dm_setup() != cudaSuccess ||
+      zgpu::kv4_attn_setup() != cudaSuccess ||
       cudaMalloc(&ctx->d_route_counter, sizeof(uint32_t)) != cudaSuccess ||
       cudaMemset(ctx->d_route_counter, 0, sizeof(uint32_t)) != cudaSuccess) {
     delete ctx;
