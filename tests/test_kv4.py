@@ -12,28 +12,28 @@ from zero_b200 import _lib
 ROOT = Path(__file__).resolve().parent.parent
 
 
-def k_bit(t, dim):
-    g, w, i = dim // 32, dim % 32 // 8, dim % 8
-    return 8 * (64 * t + 16 * g + 4 * w) + 16 * (i % 2) + 4 * (i // 2)
+def k_bits(t, dim):
+    g, c, i = dim // 32, dim % 32 // 8, dim % 8
+    return [8 * (64 * t + 16 * c + 4 * g) + 16 * (i % 2) + 4 * (i // 2) + b for b in range(4)]
 
 
-def v_bit(t, dim):
+def v_bits(t, dim):
     g, s, r = dim // 32, dim % 32 // 8, dim % 8
-    return 8 * (1024 + 512 * (t // 8) + 16 * (4 * r + t % 8 // 2) + 4 * g + 2 * (t % 2)) + 4 * s
+    at = 8 * (1024 + 512 * (t // 8) + 16 * (4 * r + t % 8 // 2) + 4 * g + 2 * (t % 2))
+    return [at + (([6, 2, 10, 14][s] + b) % 16) for b in range(4)]
 
 
 def test_tile_layout_is_a_bijection_with_whole_bytes_per_token():
     seen, owner = set(), {}
     for t in range(16):
         for dim in range(128):
-            for b in (k_bit(t, dim), v_bit(t, dim)):
-                assert b % 4 == 0 and b not in seen
+            for b in k_bits(t, dim) + v_bits(t, dim):
+                assert b not in seen
                 seen.add(b)
                 assert owner.setdefault(b // 8, t) == t
-    assert seen == set(range(0, 8 * 2048, 4))
-    ks = {2048 + 2 * (4 * t + g) for t in range(16) for g in range(4)}
-    vs = {2176 + 2 * (2 * (16 * (t // 8) + 4 * (t % 8 // 2) + g) + t % 2) for t in range(16) for g in range(4)}
-    assert ks == set(range(2048, 2176, 2)) and vs == set(range(2176, 2304, 2))
+    assert seen == set(range(8 * 2048))
+    scale = {2 * (2 * (16 * (t // 8) + 4 * (t % 8 // 2) + g) + t % 2) for t in range(16) for g in range(4)}
+    assert scale == set(range(0, 128, 2))
 
 
 def test_values_and_the_dequantising_constant_are_exact_in_binary16():

@@ -302,13 +302,17 @@ __device__ __forceinline__ uint32_t k_word_nibbles(uint32_t w, uint32_t lane) {
   if (lane & 1u) w >>= 8;
   return (w & 15u) | ((w >> 4) & 15u) << 8 | ((w >> 16) & 15u) << 4 | ((w >> 20) & 15u) << 12;
 }
-// Byte offset in a tile of lane's 16 V bits of token t, and of its V scale.
+// Byte offsets in a tile: lane's K word (shared by two lanes) and 16 V bits of
+// token t, and the scale of its group g.
 __device__ __forceinline__ uint32_t v_off(uint32_t t, uint32_t lane) {
   const uint32_t r = 4u * (lane & 1u) + ((lane >> 1) & 3u);
   return kKv4V + (t >> 3) * 512u + 16u * (4u * r + ((t & 7u) >> 1)) + 4u * (lane >> 3) + 2u * (t & 1u);
 }
-__device__ __forceinline__ uint32_t vs_off(uint32_t t, uint32_t g) {
-  return kKv4Vs + 2u * (2u * (16u * (t >> 3) + 4u * ((t & 7u) >> 1) + g) + (t & 1u));
+__device__ __forceinline__ uint32_t k_off(uint32_t t, uint32_t lane) {
+  return 64u * t + 16u * ((lane & 7u) >> 1) + 4u * (lane >> 3);
+}
+__device__ __forceinline__ uint32_t scale_off(uint32_t t, uint32_t g) {
+  return 2u * (2u * (16u * (t >> 3) + 4u * ((t & 7u) >> 1) + g) + (t & 1u));
 }
 
 constexpr uint32_t kRowWarps = 8;
@@ -334,11 +338,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
     uint32_t w = k_word_part(quantise4(kx, lane, &ks, p.status), lane);
     w |= __shfl_xor_sync(0xffffffffu, w, 1);
     const uint32_t vn = transpose_nibbles(quantise4(vx, lane, &vs, p.status), lane);
-    if (!(lane & 1u)) *reinterpret_cast<uint32_t *>(tile + 64 * t + 2 * lane) = w;
-    *reinterpret_cast<uint16_t *>(tile + v_off(t, lane)) = static_cast<uint16_t>(vn);
+    if (!(lane & 1u)) *reinterpret_cast<uint32_t *>(tile + k_off(t, lane)) = w;
+    *reinterpret_cast<uint16_t *>(tile + v_off(t, lane)) = static_cast<uint16_t>(kv4_v_bits(vn));
     if ((lane & 7u) == 0) {
-      *reinterpret_cast<__half *>(tile + kKv4Ks + 2 * (4 * t + lane / 8)) = ks;
-      *reinterpret_cast<__half *>(tile + vs_off(t, lane / 8)) = vs;
+      *reinterpret_cast<__half *>(tile + kKv4Ks + scale_off(t, lane / 8)) = ks;
+      *reinterpret_cast<__half *>(tile + kKv4Vs + scale_off(t, lane / 8)) = vs;
     }
   }
 }
@@ -361,14 +365,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4Row
       const uint8_t *tile = p.pool + kv4_tile_off(slot, head, p.n_kv, p.bt_log2);
       const uint32_t t = slot % kKv4Tile;
       if (p.k_out) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + 64 * t + 4 * (lane / 2));
-        const __half d = *reinterpret_cast<const __half *>(tile + kKv4Ks + 2 * (4 * t + lane / 8));
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + k_off(t, lane));
+        const __half d = *reinterpret_cast<const __half *>(tile + kKv4Ks + scale_off(t, lane / 8));
         kx = dequant4(k_word_nibbles(w, lane), __half2float(d));
       }
       if (p.v_out) {
         const uint32_t u = *reinterpret_cast<const uint16_t *>(tile + v_off(t, lane));
-        const __half d = *reinterpret_cast<const __half *>(tile + vs_off(t, lane / 8));
-        vx = dequant4(transpose_nibbles(u, lane), __half2float(d));
+        const __half d = *reinterpret_cast<const __half *>(tile + kKv4Vs + scale_off(t, lane / 8));
+        vx = dequant4(transpose_nibbles(kv4_v_nibbles(u), lane), __half2float(d));
       }
     } else if (slot != kKv4NoSlot && lane == 0) {
       atomicOr(p.status, ZDEV_ERR_BOUNDS);

@@ -15,17 +15,18 @@
 //
 // Storage is by tiles of 16 tokens of one kv head, 2304 contiguous bytes (one
 // bulk copy): K nibbles (1024), V nibbles (1024), K scales (128), V scales
-// (128), with q + 8 as the nibble.
-//   K: token t's row is bytes 64 t..; word w of group c (bytes 64 t + 16 c +
-//      4 w) holds dims 32 c + 8 w + 0..7, even dims in its low half and odd
-//      dims in its high half, nibble s of a half being dim pair 2 s.
+// (128), with n = q + 8 as the nibble.
+//   K: token t's row is bytes 64 t..; word g of column c (bytes 64 t + 16 c +
+//      4 g) holds dims 32 g + 8 c + 0..7, even dims in its low half and odd
+//      dims in its high half, bits 4 s of a half being dim pair 2 s.
 //   V: half p = t / 8, column c = (t % 8) / 2, odd = t % 2; the 16 bits at
-//      512 p + 16 (4 r + c) + 4 g + 2 odd hold dims 32 g + 8 s + r, s = 0..3.
-//   K scales: half index 4 t + c.  V scales: half index 2 (16 p + 4 c + g) + odd.
+//      512 p + 16 (4 r + c) + 4 g + 2 odd hold dims 32 g + 8 s + r, s = 0..3:
+//      s = 0 at bits 6..9, 1 at 2..5, 2 at 10..13, 3 at 14, 15, 0, 1 (after a
+//      swap of the two bytes, 2 is at 2..5 and 3 at 6..9).
+//   Scales of K and of V: half index 2 (16 p + 4 c + g) + odd.
 // These are the m16n8k16 B fragments: lane (r, c) = (lane / 4, lane % 4) of a
 // warp reads its K words of 8 tokens, or its V words of 16, with one 16-byte
-// shared-memory load per 512 bytes, and one shift, one logical operation and
-// one half2 fma give two operand values.  Every byte belongs to one token, so
+// shared-memory load per 512 bytes.  Every byte belongs to one token, so
 // tokens are stored without touching their neighbours.
 #pragma once
 
@@ -52,6 +53,14 @@ constexpr float kKv4MaxScale = 2720.f;
 __host__ __device__ inline size_t kv4_tile_off(uint32_t slot, uint32_t head, uint32_t n_kv, uint32_t bt_log2) {
   const uint32_t block = slot >> bt_log2, tile = (slot & ((1u << bt_log2) - 1u)) / kKv4Tile;
   return (((static_cast<size_t>(block) * n_kv + head) << (bt_log2 - 4)) + tile) * kKv4TileBytes;
+}
+
+// A token's 16 bits of V from nibbles s at bits 4 s, and back.
+__host__ __device__ inline uint32_t kv4_v_bits(uint32_t n) {
+  return (n & 15u) << 6 | ((n >> 4) & 15u) << 2 | ((n >> 8) & 15u) << 10 | ((n >> 12) & 3u) << 14 | (n >> 14);
+}
+__host__ __device__ inline uint32_t kv4_v_nibbles(uint32_t v) {
+  return ((v >> 6) & 15u) | ((v >> 2) & 15u) << 4 | ((v >> 10) & 15u) << 8 | ((v >> 14) | (v & 3u) << 2) << 12;
 }
 
 // Element types of rows given to append / gather / attention.

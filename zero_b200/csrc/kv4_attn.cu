@@ -14,20 +14,28 @@
 //   values whose sum holds 22 bits, in rows r and r + 8 of the fragment.  The
 //   cache's values are exact in binary16, so q K^T and P V keep f32 accuracy
 //   at the price of eight rows instead of sixteen, which a memory-bound
-//   kernel has to spare; both halves of a sum land in one thread.  A query
-//   row is scaled by a power of two first (its largest value in [1, 2)), so
-//   neither half leaves binary16's range; P is held times 2^15, which keeps
-//   probabilities down to 2^-39 of the row's largest.
+//   kernel has to spare; both halves of a score land in one thread.  P V is
+//   taken transposed, V^T P^T: the scores' fragment is P^T's as it stands, the
+//   values are the sixteen rows, and the result takes half the registers.  For
+//   16-bit rows P is one binary16 value, 11 bits.  A query
+//   row is scaled by a power of two first (its largest value in [256, 512)),
+//   so neither half leaves binary16's range; P is held times 2^15, which
+//   keeps probabilities down to 2^-39 of the row's largest.
 //
-//   Loads.  Each warp streams its own tiles (16 keys, 2304 contiguous bytes)
+//   Keys stay integers: a masked nibble is a subnormal binary16, n 2^-24 (16
+//   times that at bits 4..7, which the query's other half carries as 1 / 16),
+//   so a value pair costs one logical operation.  Each group of 32 dims has
+//   its own sum, sum_g d_g (sum_j q_j n_j - 8 sum_j q_j), scaled in f32.
+//   Values are made binary16 by the bits' place: under a fixed exponent a
+//   nibble is a constant plus n, and (16 + n) d - 24 d is one exact fma since
+//   24 d is exact; for 256 + n an add takes the constant off first.
+//
+//   Loads.  Each warp streams its own units (32 keys, two tiles of 2304 bytes)
 //   through a private ring of bulk copies, one mbarrier a stage, and no
-//   barrier joins the warps until a piece of work ends.  The tile's layout is
-//   the fragment's (kv4.h): 16-byte shared loads without bank conflicts, and
-//   per two values a shift, a logical operation and one half2 fma:
-//   (16 + n) d - 24 d = (n - 8) d, exact because 24 d is.
+//   barrier joins the warps until a piece of work ends.
 //
 //   Split.  All pieces of work (sequence, kv head, eight rows) are laid end to
-//   end in units of one tile and cut into equal ranges, one per CTA, so a
+//   end in units of 32 keys and cut into equal ranges, one per CTA, so a
 //   ragged batch or one long sequence keeps every SM equally busy.  A piece
 //   cut by a range boundary leaves unnormalised partials (max, sum, o) in the
 //   workspace; the CTA that arrives last merges them in range order, so the
@@ -43,18 +51,24 @@ namespace {
 
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kCtasPerSm = 2;
-constexpr uint32_t kStages = 4;                  // tiles in flight per warp
+constexpr uint32_t kUnit = 2 * kKv4Tile;         // keys a warp takes at a time
+constexpr uint32_t kUnitBytes = 2 * kKv4TileBytes;
+constexpr uint32_t kStages = 2;                  // units in flight per warp
 constexpr uint32_t kRows = 8;                    // query rows of a piece
 constexpr uint32_t kPartFloats = kRows * (kKv4Head + 2);   // o, max, sum
+constexpr uint32_t kMergeRow = kKv4Head + 4;     // floats between a warp's rows: its stores hit 32 banks
+constexpr uint32_t kMergeFloats = kRows * (kMergeRow + 2);
 constexpr float kPShift = 15.f;                  // P is held times 2^15
-constexpr uint32_t kMinTiles = kWarps;           // a range is worth a tile per warp
+constexpr uint32_t kMinUnits = kWarps / 2;       // a range is worth a unit for every second warp
 
 // Dynamic shared memory: the warps' rings, the warps' partials, the sums of
 // work over the sequences.
-constexpr uint32_t kRingBytes = kWarps * kStages * kKv4TileBytes;
-constexpr uint32_t kMergeBytes = kWarps * kPartFloats * 4;
+constexpr uint32_t kRingBytes = kWarps * kStages * kUnitBytes;
+constexpr uint32_t kMergeBytes = kWarps * kMergeFloats * 4;
+constexpr uint32_t kQBytes = 8 * 512;            // hi and lo of eight rows, as fragments
 constexpr uint32_t kOffMerge = kRingBytes;
-constexpr uint32_t kOffSums = kOffMerge + kMergeBytes;
+constexpr uint32_t kOffQ = kOffMerge + kMergeBytes;
+constexpr uint32_t kOffSums = kOffQ + kQBytes;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -73,24 +87,40 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Nibble s of both halves of w as (n - 8) d: the nibble becomes bits 6..9 of
-// a binary16 with 16's exponent, 16 + n.
-template <int S>
-__device__ __forceinline__ uint32_t dequant2(uint32_t w, __half2 d, __half2 m24d) {
-  const uint32_t sh = S == 0 ? w << 6 : S == 1 ? w << 2 : S == 2 ? w >> 2 : w >> 6;
-  const uint32_t x = (sh & 0x03C003C0u) | 0x4C004C00u;
-  return h2bits(__hfma2(bits2h(x), d, m24d));
-}
-
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
+
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// The exponents of 16 and 256, read back from shared memory so that they stay
+// in registers: a logical operation takes one constant, and where both
+// operands are known the compiler makes two operations of it.
+struct Magic {
+  uint32_t x16, x256;
+};
+__device__ __forceinline__ Magic magic(uint32_t saddr) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(saddr), "r"(0x4C004C00u), "r"(0x5C005C00u) : "memory");
+  Magic g;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(g.x16), "=r"(g.x256) : "r"(saddr) : "memory");
+  return g;
+}
+// The four V nibbles of both halves of w as (n - 8) d, exactly.
+__device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, const Magic &g, uint32_t (&v)[4]) {
+  const uint32_t x = __byte_perm(w, 0u, 0x2301u);
+  const __half2 m264 = __half2half2(__ushort_as_half(0xDC20));
+  v[0] = h2bits(__hfma2(bits2h((w & 0x03C003C0u) | g.x16), d, m24d));
+  v[1] = h2bits(__hmul2(__hadd2(bits2h((w & 0x003C003Cu) | g.x256), m264), d));
+  v[2] = h2bits(__hmul2(__hadd2(bits2h((x & 0x003C003Cu) | g.x256), m264), d));
+  v[3] = h2bits(__hfma2(bits2h((x & 0x03C003C0u) | g.x16), d, m24d));
 }
 
 template <class T>
@@ -143,28 +173,28 @@ __device__ __forceinline__ Seq load_seq(const Kv4AttnParams &p, uint32_t i, bool
   return s;
 }
 
-struct WarpState {
-  float o[16][4];
-  float m, l;
-};
-
 template <class T>
 __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const Kv4AttnParams p) {
+  // a 16-bit row is exact as hi alone, and so near enough is a probability
+  // that a 16-bit result is made of
+  constexpr bool kLo = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps * kStages];
   __shared__ uint64_t s_scan[kWarps];
-  __shared__ uint32_t s_last;
+  __shared__ uint32_t s_last, s_limit[kRows];
+  __shared__ float s_scl[kRows], s_bias[kRows][4];
+  __shared__ __align__(8) uint32_t s_magic[2];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffSums);   // work before sequence i, n_seq + 1
   float *merge = reinterpret_cast<float *>(smem + kOffMerge);
-  const uint32_t ring = smem_addr(smem) + warp * kStages * kKv4TileBytes;
+  const uint32_t ring = smem_addr(smem) + warp * kStages * kUnitBytes;
   const uint32_t bar0 = smem_addr(&bars[warp * kStages]);
 
   if (lane == 0) {
     for (uint32_t s = 0; s < kStages; ++s) mbar_init(bar0 + 8 * s, 1);
     fence_barrier_init();
   }
-  // work of sequence i: kv heads x pieces of eight rows x tiles
+  // work of sequence i: kv heads x pieces of eight rows x units
   {
     uint64_t base = 0;
     bool bad = false, blind = false;
@@ -174,7 +204,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       if (i < p.n_seq) {
         const Seq s = load_seq(p, i, &bad);
         blind |= s.len < s.nq;
-        w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * ((s.len + kKv4Tile - 1) / kKv4Tile);
+        w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * ((s.len + kUnit - 1) / kUnit);
       }
       uint64_t inc = w;
 #pragma unroll
@@ -208,7 +238,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   }
 
   const uint64_t W = sums[p.n_seq];
-  uint64_t G = (W + kMinTiles - 1) / kMinTiles;
+  uint64_t G = (W + kMinUnits - 1) / kMinUnits;
   if (G > gridDim.x) G = gridDim.x;
   if (blockIdx.x >= G) return;
   uint64_t at = W * blockIdx.x / G;
@@ -223,171 +253,220 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     }
     seq = lo;
   }
-  uint32_t it0 = 0;         // tiles that this warp took before the piece: stage and phase of the ring
+  uint32_t it0 = 0;         // units that this warp took before the piece: stage and phase of the ring
   bool dead = false;        // a wait of this warp ran out
+  const Magic mg = magic(smem_addr(s_magic));
 
   while (at < end) {
     while (sums[seq + 1] <= at) ++seq;
     bool bad = false;
     const Seq s = load_seq(p, seq, &bad);
-    const uint32_t n_tiles = (s.len + kKv4Tile - 1) / kKv4Tile;
+    const uint32_t n_units = (s.len + kUnit - 1) / kUnit;
     const uint32_t pieces = (s.nq * p.group + kRows - 1) / kRows;
-    const uint64_t piece = (at - sums[seq]) / n_tiles;
-    const uint64_t piece_at = sums[seq] + piece * n_tiles;   // the piece in units of work
+    const uint64_t piece = (at - sums[seq]) / n_units;
+    const uint64_t piece_at = sums[seq] + piece * n_units;   // the piece in units of work
     const uint32_t head = static_cast<uint32_t>(piece / pieces), rt = static_cast<uint32_t>(piece % pieces);
     const uint32_t t0 = static_cast<uint32_t>(at - piece_at);
-    const uint32_t t1 = static_cast<uint32_t>(end - piece_at < n_tiles ? end - piece_at : n_tiles);
+    const uint32_t t1 = static_cast<uint32_t>(end - piece_at < n_units ? end - piece_at : n_units);
     const uint32_t *table = p.table + static_cast<size_t>(seq) * p.table_width;
     const uint32_t tpb_log2 = p.bt_log2 - 4;
-    // this warp's tiles: t0 + warp + 8 k, k < nk
+    // this warp's units: t0 + warp + 8 k, k < nk
     const uint32_t nk = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;
 
-    // blocks of the next 32 tiles to be copied, one per lane, and of the 32 after
-    auto entry = [&](uint32_t k) -> uint32_t {
-      return k < nk ? __ldg(table + ((t0 + warp + kWarps * k) >> tpb_log2)) : 0u;
+    // Where the next units lie: lane i holds the address of unit k0 + i, or
+    // with blocks of 16 tokens lanes 2 i and 2 i + 1 those of unit k0 + i's
+    // tiles, and the lane that holds an address issues its copy.  Table
+    // entries are fetched a batch ahead of the addresses.
+    const bool split = tpb_log2 == 0;
+    const uint32_t batch = split ? 16 : 32;
+    auto tile_of = [&](uint32_t k0) { return 2 * (t0 + warp + kWarps * (k0 + (split ? lane >> 1 : lane))) + (split ? lane & 1u : 0u); };
+    auto entry = [&](uint32_t k0) -> uint32_t {
+      const uint32_t tile = tile_of(k0);
+      return k0 + (split ? lane >> 1 : lane) < nk && tile * kKv4Tile < s.len ? __ldg(table + (tile >> tpb_log2)) : kKv4NoSlot;
     };
-    uint32_t ent = entry(lane), ent_next = entry(32 + lane), issued = 0;
-    uint32_t bad_block = 0;      // bit k % 32 of the tiles in flight
+    const uint8_t *src = nullptr;
+    uint32_t ent = entry(0), issued = 0;
+    // units of this batch and the one before with a block outside the pool
+    uint32_t bad_now = 0, bad_before = 0;
+    auto addresses = [&](uint32_t k0) {
+      const uint32_t tile = tile_of(k0);
+      const bool is = k0 + (split ? lane >> 1 : lane) < nk && tile * kKv4Tile < s.len, ok = ent < p.n_blocks;
+      // a tile that is not there is copied from block 0, for the mask to drop
+      src = p.pool + (((static_cast<size_t>(ok ? ent : 0u) * p.n_kv + head) << tpb_log2) + (tile & ((1u << tpb_log2) - 1u))) *
+                         kKv4TileBytes;
+      bad_before = bad_now;
+      bad_now = __ballot_sync(0xffffffffu, is && !ok);
+      if (is && !ok) atomicOr(p.status, ZDEV_ERR_BOUNDS);
+      ent = entry(k0 + batch);
+    };
     auto issue = [&]() {
-      const uint32_t k = issued, tile = t0 + warp + kWarps * k;
-      const uint32_t block = __shfl_sync(0xffffffffu, ent, k & 31u);
-      const uint32_t stage = (it0 + k) % kStages, bar = bar0 + 8 * stage, dst = ring + stage * kKv4TileBytes;
-      const bool ok = block < p.n_blocks;
-      if (lane == 0) {
-        if (ok) {
-          const uint8_t *src =
-              p.pool + (((static_cast<size_t>(block) * p.n_kv + head) << tpb_log2) + (tile & ((1u << tpb_log2) - 1u))) *
-                           kKv4TileBytes;
-          mbar_arrive_expect_tx(bar, kKv4TileBytes);
-          bulk_copy_g2s(dst, src, kKv4TileBytes, bar);
-        } else {
-          mbar_arrive(bar);
-          atomicOr(p.status, ZDEV_ERR_BOUNDS);
-        }
+      const uint32_t i = issued & (batch - 1);
+      if (i == 0) addresses(issued);
+      const uint32_t stage = (it0 + issued) % kStages, bar = bar0 + 8 * stage, dst = ring + stage * kUnitBytes;
+      if (split) {
+        if (lane == 2 * i) mbar_arrive_expect_tx(bar, kUnitBytes);
+        __syncwarp();
+        if ((lane >> 1) == i) bulk_copy_g2s(dst + (lane & 1u) * kKv4TileBytes, src, kKv4TileBytes, bar);
+      } else if (lane == i) {
+        mbar_arrive_expect_tx(bar, kUnitBytes);
+        bulk_copy_g2s(dst, src, kUnitBytes, bar);
       }
-      bad_block = (bad_block & ~(1u << (k & 31u))) | (ok ? 0u : 1u << (k & 31u));
       ++issued;
-      if ((issued & 31u) == 0) {
-        ent = ent_next;
-        ent_next = entry(issued + 32 + lane);
-      }
     };
     const uint32_t ahead = nk < kStages ? nk : kStages;
     if (!dead)
       while (issued < ahead) issue();
 
-    // the queries: row r of the piece, dims 32 c .. 32 c + 31, hi and lo
-    const uint32_t row = rt * kRows + r, n_rows = s.nq * p.group;
-    const uint32_t tok = row < n_rows ? row / p.group : 0, hd = row < n_rows ? row % p.group : 0;
-    uint32_t qh[8][2], ql[8][2];
-    float scl;
+    // the queries: warp w takes row w of the piece, four dims per lane, scaled
+    // by a power of two and split in hi and lo; fragment kk of lane (r, c) is
+    // the 16 bytes at 512 kk + 16 lane: dims 32 (kk / 2) + 8 c + 4 (kk % 2) + 0..3
+    const uint32_t n_rows = s.nq * p.group;
     {
-      const T *qp = static_cast<const T *>(p.q) + (s.q0 + tok) * p.q_stride +
-                    (static_cast<size_t>(head) * p.group + hd) * kKv4Head + 32 * c;
-      float4 x[8];
-      float amax = 0.f;
+      const uint32_t row = rt * kRows + warp, tok = row < n_rows ? row / p.group : 0, hd = row < n_rows ? row % p.group : 0;
+      const float4 x = q4(static_cast<const T *>(p.q) + (s.q0 + tok) * p.q_stride +
+                          (static_cast<size_t>(head) * p.group + hd) * kKv4Head + 4 * lane);
+      float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[k] = q4(qp + 4 * k);
-        amax = fmaxf(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))), amax);
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      for (int off = 1; off < 32; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      // 256 times: the pairs that meet 16 n are held / 16, their low halves
+      // still far from binary16's subnormals
       int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-      e = e < -100 ? -100 : e > 126 ? 126 : e;
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      scl = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      e = e < -100 ? -100 : e > 110 ? 110 : e;
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23), down16 = down * 0.0625f;
+      const float4 y = make_float4(x.x * down, x.y * down, x.z * down16, x.w * down16);
+      const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
+      const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+      *reinterpret_cast<uint4 *>(smem + kOffQ + 512 * (2 * (lane >> 3) + (lane & 1u)) + 16 * (4 * warp + ((lane & 7u) >> 1))) =
+          make_uint4(h2bits(h0), h2bits(__floats2half2_rn(y.x - f0.x, y.y - f0.y)), h2bits(h1),
+                     h2bits(__floats2half2_rn(y.z - f1.x, y.w - f1.y)));
+      // - 8 sum q of each group, in the units of the products
+      float qsum = (y.x + y.y) + 16.f * (y.z + y.w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float y[4] = {x[k].x * down, x[k].y * down, x[k].z * down, x[k].w * down};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const __half2 hi = __floats2half2_rn(y[2 * h], y[2 * h + 1]);
-          const float2 f = __half22float2(hi);
-          qh[k][h] = h2bits(hi);
-          ql[k][h] = h2bits(__floats2half2_rn(y[2 * h] - f.x, y[2 * h + 1] - f.y));
-        }
+      for (int off = 1; off < 8; off <<= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
+      if ((lane & 7u) == 0) s_bias[warp][lane >> 3] = qsum * (-8.f * 0x1p-24f);
+      if (lane == 0) {
+        // keys that the row sees: 0 .. limit - 1 (none when its position is negative)
+        const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + tok + 1;
+        // a row behind the last is the first one again, for no use
+        s_limit[warp] = pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
+        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + 24 - 8 + e) << 23);
       }
     }
-    // keys that row r sees: 0 .. limit - 1 (none when its position is negative)
-    const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + tok + 1;
-    const uint32_t limit = row < n_rows && pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
-
-    WarpState st;
-    st.m = -INFINITY;
-    st.l = 0.f;
+    __syncthreads();
+    const uint32_t limit = s_limit[r], qs = smem_addr(smem) + kOffQ + 16 * lane;
+    const float scl = s_scl[r];
+    uint32_t all_see = limit;       // keys that every row sees need no mask
 #pragma unroll
-    for (int n = 0; n < 16; ++n) st.o[n][0] = st.o[n][1] = st.o[n][2] = st.o[n][3] = 0.f;
+    for (int off = 4; off < 32; off <<= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, off));
+
+    float bias[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) bias[g] = s_bias[r][g];
+
+    // o[n]: dims 16 n + r (and + 8) of rows 2 c and 2 c + 1; m, l: row r
+    float o[8][4], m = -INFINITY;
+    float2 l = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
     for (uint32_t k = 0; k < nk && !dead; ++k) {
-      const uint32_t stage = (it0 + k) % kStages, base = ring + stage * kKv4TileBytes;
+      const uint32_t stage = (it0 + k) % kStages;
       dead = __any_sync(0xffffffffu, !mbar_wait(bar0 + 8 * stage, ((it0 + k) / kStages) & 1u, p.status));
       if (dead) {       // the copies in flight land before the CTA may end
-        for (++k; k < issued; ++k) mbar_wait(bar0 + 8 * ((it0 + k) % kStages), ((it0 + k) / kStages) & 1u, p.status);
+        for (uint32_t x = k + 1; x < issued; ++x)
+          mbar_wait(bar0 + 8 * ((it0 + x) % kStages), ((it0 + x) / kStages) & 1u, p.status);
         break;
       }
-      const uint32_t key0 = (t0 + warp + kWarps * k) * kKv4Tile;
-      if (!((bad_block >> (k & 31u)) & 1u)) {
-        float sc[2][4];
+      const uint32_t base0 = ring + stage * kUnitBytes, key0 = (t0 + warp + kWarps * k) * kUnit;
+      // scores of keys 8 u + 2 c and + 1 of row r
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 kw[2], kd[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint4 w = lds128(base + 512 * u + 16 * lane);
-          const uint32_t dw = lds16(base + kKv4Ks + 64 * u + 2 * lane);
-          const __half2 d = bits2h(dw | dw << 16), m24 = __hmul2(d, __float2half2_rn(-24.f));
-          sc[u][0] = sc[u][1] = sc[u][2] = sc[u][3] = 0.f;
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          kw[u] = lds128(base0 + kKv4TileBytes * h + 512 * u + 16 * lane);
+          kd[u] = lds128(base0 + kKv4TileBytes * h + kKv4Ks + 64 * u + 16 * c);
+        }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma16816(sc[u], qh[2 * j][0], ql[2 * j][0], qh[2 * j][1], ql[2 * j][1], dequant2<0>(ww[j], d, m24),
-                     dequant2<1>(ww[j], d, m24));
-            mma16816(sc[u], qh[2 * j + 1][0], ql[2 * j + 1][0], qh[2 * j + 1][1], ql[2 * j + 1][1],
-                     dequant2<2>(ww[j], d, m24), dequant2<3>(ww[j], d, m24));
+        for (int g = 0; g < 4; ++g) {
+          const uint4 qa = lds128(qs + 1024 * g), qb = lds128(qs + 1024 * g + 512);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t w = g == 0 ? kw[u].x : g == 1 ? kw[u].y : g == 2 ? kw[u].z : kw[u].w, w8 = w >> 8;
+            const uint32_t dw = g == 0 ? kd[u].x : g == 1 ? kd[u].y : g == 2 ? kd[u].z : kd[u].w;
+            float sc[4];
+            mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, w & 0x000F000Fu, w & 0x00F000F0u);
+            mma16816(sc, qb.x, qb.y, qb.z, qb.w, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+            const float2 t = add2_rn(add2_rn(make_float2(sc[0], sc[1]), make_float2(sc[2], sc[3])),
+                                     make_float2(bias[g], bias[g]));
+            v[2 * h + u] = fma2_rn(t, __half22float2(bits2h(dw)), v[2 * h + u]);
           }
         }
-        float v[4];
-        float mx = st.m;
+      }
+      float mx = m;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 4; ++u) v[u] = mul2_rn(v[u], make_float2(scl, scl));
+      if (key0 + kUnit > all_see || (bad_now | bad_before)) {
+        // which of the unit's tiles lie in the pool: its batch is the last
+        // one addressed or, with units in flight, the one before
+        const uint32_t bm = (issued - 1) / batch == k / batch ? bad_now : bad_before, i = k & (batch - 1);
+        const bool gone0 = (bm >> (split ? 2 * i : i)) & 1u, gone1 = (bm >> (split ? 2 * i + 1 : i)) & 1u;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t key = key0 + 8 * u + 2 * c + e;
-            v[2 * u + e] = key < limit ? (sc[u][e] + sc[u][2 + e]) * scl : -INFINITY;
-            mx = fmaxf(mx, v[2 * u + e]);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float ms = mx == -INFINITY ? 0.f : mx;
-        if (__any_sync(0xffffffffu, mx > st.m)) {
-          const float a = ex2(st.m - ms);
-          st.l *= a;
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[n][e] *= a;
-          st.m = mx;
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t key = key0 + 8 * u + 2 * c;
+          if (key >= limit || (u < 2 ? gone0 : gone1)) v[u].x = -INFINITY;
+          if (key + 1 >= limit || (u < 2 ? gone0 : gone1)) v[u].y = -INFINITY;
         }
-        uint32_t ph[2], pl[2];
+      }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float p0 = ex2(v[2 * u] - (ms - kPShift)), p1 = ex2(v[2 * u + 1] - (ms - kPShift));
-          st.l += p0 + p1;
-          const __half2 hi = __floats2half2_rn(p0, p1);
-          const float2 f = __half22float2(hi);
-          ph[u] = h2bits(hi);
-          pl[u] = h2bits(__floats2half2_rn(p0 - f.x, p1 - f.y));
+      for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fmaxf(v[u].x, v[u].y));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float ms = mx == -INFINITY ? 0.f : mx;
+      if (__any_sync(0xffffffffu, mx > m)) {
+        const float a = ex2(m - ms);
+        const float2 aa = make_float2(__shfl_sync(0xffffffffu, a, 8 * c), __shfl_sync(0xffffffffu, a, 8 * c + 4));
+        l = mul2_rn(l, make_float2(a, a));
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const float2 x = mul2_rn(make_float2(o[n][0], o[n][1]), aa), y = mul2_rn(make_float2(o[n][2], o[n][3]), aa);
+          o[n][0] = x.x, o[n][1] = x.y, o[n][2] = y.x, o[n][3] = y.y;
         }
-        const uint4 w0 = lds128(base + kKv4V + 16 * lane), w1 = lds128(base + kKv4V + 512 + 16 * lane);
-        const uint4 d0 = lds128(base + kKv4Vs + 16 * c), d1 = lds128(base + kKv4Vs + 64 + 16 * c);
+        m = mx;
+      }
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float2 e = add2_rn(v[u], make_float2(kPShift - ms, kPShift - ms)), pr = make_float2(ex2(e.x), ex2(e.y));
+        l = add2_rn(l, pr);
+        const __half2 hi = __floats2half2_rn(pr.x, pr.y);
+        ph[u] = h2bits(hi);
+        if (kLo) {
+          const float2 lo = sub2_rn(pr, __half22float2(hi));
+          pl[u] = h2bits(__floats2half2_rn(lo.x, lo.y));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t b = base0 + kKv4TileBytes * t + kKv4V;
+        const uint4 w0 = lds128(b + 16 * lane), w1 = lds128(b + 512 + 16 * lane);
+        const uint4 d0 = lds128(b + kKv4Vs - kKv4V + 16 * c), d1 = lds128(b + kKv4Vs - kKv4V + 64 + 16 * c);
         const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
         const uint32_t e0[4] = {d0.x, d0.y, d0.z, d0.w}, e1[4] = {d1.x, d1.y, d1.z, d1.w};
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const __half2 x0 = bits2h(e0[g]), x1 = bits2h(e1[g]);
-          const __half2 y0 = __hmul2(x0, __float2half2_rn(-24.f)), y1 = __hmul2(x1, __float2half2_rn(-24.f));
-          mma16816(st.o[4 * g], ph[0], pl[0], ph[1], pl[1], dequant2<0>(a0[g], x0, y0), dequant2<0>(a1[g], x1, y1));
-          mma16816(st.o[4 * g + 1], ph[0], pl[0], ph[1], pl[1], dequant2<1>(a0[g], x0, y0), dequant2<1>(a1[g], x1, y1));
-          mma16816(st.o[4 * g + 2], ph[0], pl[0], ph[1], pl[1], dequant2<2>(a0[g], x0, y0), dequant2<2>(a1[g], x1, y1));
-          mma16816(st.o[4 * g + 3], ph[0], pl[0], ph[1], pl[1], dequant2<3>(a0[g], x0, y0), dequant2<3>(a1[g], x1, y1));
+          uint32_t v0[4], v1[4];
+          v_values(a0[g], x0, __hmul2(x0, __float2half2_rn(-24.f)), mg, v0);
+          v_values(a1[g], x1, __hmul2(x1, __float2half2_rn(-24.f)), mg, v1);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            mma16816(o[2 * g + n], v0[2 * n], v0[2 * n + 1], v1[2 * n], v1[2 * n + 1], ph[2 * t], ph[2 * t + 1]);
+            if (kLo) mma16816(o[2 * g + n], v0[2 * n], v0[2 * n + 1], v1[2 * n], v1[2 * n + 1], pl[2 * t], pl[2 * t + 1]);
+          }
         }
       }
       __syncwarp();       // every lane has read the stage before it is filled again
@@ -396,16 +475,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     it0 += nk;
 
     // the warps' states, then the piece
-    st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-    st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-    float *mine = merge + warp * kPartFloats;
+    float lsum = l.x + l.y;
+    lsum += __shfl_xor_sync(0xffffffffu, lsum, 1);
+    lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
+    float *mine = merge + warp * kMergeFloats;
 #pragma unroll
-    for (int n = 0; n < 16; ++n)
-      *reinterpret_cast<float2 *>(mine + r * kKv4Head + 8 * n + 2 * c) =
-          make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(2 * c + (e & 1)) * kMergeRow + 16 * n + 8 * (e >> 1) + r] = o[n][e];
     if (c == 0) {
-      mine[kRows * kKv4Head + 2 * r] = st.m;
-      mine[kRows * kKv4Head + 2 * r + 1] = st.l;
+      mine[kRows * kMergeRow + 2 * r] = m;
+      mine[kRows * kMergeRow + 2 * r + 1] = lsum;
     }
     __syncthreads();
     // thread: row mr, dims 4 mc ..
@@ -424,11 +504,11 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     };
 #pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) {
-      const float *src = merge + w * kPartFloats;
-      fold(src[kRows * kKv4Head + 2 * mr], src[kRows * kKv4Head + 2 * mr + 1],
-           *reinterpret_cast<const float4 *>(src + mr * kKv4Head + 4 * mc));
+      const float *src = merge + w * kMergeFloats;
+      fold(src[kRows * kMergeRow + 2 * mr], src[kRows * kMergeRow + 2 * mr + 1],
+           *reinterpret_cast<const float4 *>(src + mr * kMergeRow + 4 * mc));
     }
-    bool whole = t0 == 0 && t1 == n_tiles;
+    bool whole = t0 == 0 && t1 == n_units;
     if (!whole) {
       float *dst = p.part + (2ull * blockIdx.x + (t0 == 0 ? 1 : 0)) * kPartFloats;
       *reinterpret_cast<float4 *>(dst + mr * kKv4Head + 4 * mc) = O;
@@ -440,7 +520,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       __syncthreads();
       // the ranges that share the piece
       const uint32_t c0 = static_cast<uint32_t>(((piece_at + 1) * G - 1) / W);
-      const uint32_t c1 = static_cast<uint32_t>(((piece_at + n_tiles) * G - 1) / W);
+      const uint32_t c1 = static_cast<uint32_t>(((piece_at + n_units) * G - 1) / W);
       if (tid == 0) {
         const uint32_t n = atomicAdd(&p.counters[c0], 1u);
         s_last = n == c1 - c0;
@@ -449,14 +529,38 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       __syncthreads();
       if (s_last) {
         __threadfence();
+        // the row's largest maximum and the ranges' weights, a lane each, then
+        // the sums: the loads of a batch do not wait for one another
         M = -INFINITY;
         L = 0.f;
         O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (uint32_t k = c0; k <= c1; ++k) {
-          const float *src = p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats;
-          fold(__ldcg(src + kRows * kKv4Head + 2 * mr), __ldcg(src + kRows * kKv4Head + 2 * mr + 1),
-               __ldcg(reinterpret_cast<const float4 *>(src + mr * kKv4Head + 4 * mc)));
+        for (uint32_t k0 = c0; k0 <= c1; k0 += 32) {
+          const uint32_t k = k0 + mc;
+          float pm = -INFINITY, pl = 0.f;
+          if (k <= c1) {
+            const float *src = p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats + kRows * kKv4Head + 2 * mr;
+            pm = __ldcg(src);
+            pl = __ldcg(src + 1);
+          }
+          float nm = fmaxf(M, pm);
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, off));
+          const float keep = nm == -INFINITY ? 1.f : ex2(M - nm);
+          // a range that saw no key has nothing to add; a broken one (a NaN sum) has
+          const float w = pm == -INFINITY && pl == 0.f ? 0.f : ex2(pm - nm);
+          L *= keep;
+          O.x *= keep, O.y *= keep, O.z *= keep, O.w *= keep;
+          const uint32_t n = min(32u, c1 - k0 + 1);
+#pragma unroll 8
+          for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t kj = k0 + j;
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(
+                p.part + (2ull * kj + (kj == c0 ? 1 : 0)) * kPartFloats + mr * kKv4Head + 4 * mc));
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            L += __shfl_sync(0xffffffffu, pl, j) * wj;
+            O.x += x.x * wj, O.y += x.y * wj, O.z += x.z * wj, O.w += x.w * wj;
+          }
+          M = nm;
         }
         whole = true;
       }
