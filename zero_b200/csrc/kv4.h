@@ -102,15 +102,21 @@ struct Kv4AttnParams {
   const uint32_t *starts, *kv_lens, *table;
   uint32_t table_width, n_seq, n_rows, max_q, n_kv, group, n_blocks, bt_log2;
   float scale;
-  float *part;                // partial slots of the CTAs
+  float *part;                // partial slots of the launch's CTAs
   uint32_t *counters;         // zero between calls
+  uint32_t few_only;          // kv4_attn.cu: sequences of more rows go to kv4_prompt.cu
   uint32_t *status;
 };
-// Bytes of the partials and the number of counters a device needs.
+// Bytes of the partials and the number of counters a workspace needs.
 size_t kv4_attn_part_bytes(int sm_count);
 uint32_t kv4_attn_counters(int sm_count);
 cudaError_t kv4_attn_setup();
 cudaError_t launch_kv4_attention(const Kv4AttnParams &p, Kv4Type t, int sm_count, uint32_t *launches, cudaStream_t s);
+// The part of it for sequences with many query rows (kv4_prompt.cu).
+size_t kv4_prompt_part_bytes(int sm_count);
+uint32_t kv4_prompt_counters(int sm_count);
+cudaError_t kv4_prompt_setup();
+cudaError_t launch_kv4_prompt(const Kv4AttnParams &p, Kv4Type t, int sm_count, cudaStream_t s);
 
 }  // namespace zgpu
 

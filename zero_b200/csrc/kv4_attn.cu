@@ -4,7 +4,8 @@
 // own position: row i's queries are its last ones, query t of n at position
 // kv_len - n + t.
 //
-// kv4_rows_kernel: few query rows per kv head (decode, short continuations).
+// kv4_rows_kernel: at most 16 query rows per kv head (decode, short
+// continuations); kv4_prompt.cu takes the sequences with more.
 // Bound by the cache read, 144 bytes per key and kv head, and close behind it
 // by instruction issue: unpacking 256 values per key and head.
 //
@@ -40,10 +41,7 @@
 //   cut by a range boundary leaves unnormalised partials (max, sum, o) in the
 //   workspace; the CTA that arrives last merges them in range order, so the
 //   result does not depend on which one that is.
-#include <cuda_bf16.h>
-
-#include "common.cuh"
-#include "kv4.h"
+#include "kv4_rows.cuh"
 
 namespace zgpu {
 
@@ -70,15 +68,6 @@ constexpr uint32_t kOffMerge = kRingBytes;
 constexpr uint32_t kOffQ = kOffMerge + kMergeBytes;
 constexpr uint32_t kOffSums = kOffQ + kQBytes;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 bits2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -99,78 +88,6 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// The exponents of 16 and 256, read back from shared memory so that they stay
-// in registers: a logical operation takes one constant, and where both
-// operands are known the compiler makes two operations of it.
-struct Magic {
-  uint32_t x16, x256;
-};
-__device__ __forceinline__ Magic magic(uint32_t saddr) {
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(saddr), "r"(0x4C004C00u), "r"(0x5C005C00u) : "memory");
-  Magic g;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(g.x16), "=r"(g.x256) : "r"(saddr) : "memory");
-  return g;
-}
-// The four V nibbles of both halves of w as (n - 8) d, exactly.
-__device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, const Magic &g, uint32_t (&v)[4]) {
-  const uint32_t x = __byte_perm(w, 0u, 0x2301u);
-  const __half2 m264 = __half2half2(__ushort_as_half(0xDC20));
-  v[0] = h2bits(__hfma2(bits2h((w & 0x03C003C0u) | g.x16), d, m24d));
-  v[1] = h2bits(__hmul2(__hadd2(bits2h((w & 0x003C003Cu) | g.x256), m264), d));
-  v[2] = h2bits(__hmul2(__hadd2(bits2h((x & 0x003C003Cu) | g.x256), m264), d));
-  v[3] = h2bits(__hfma2(bits2h((x & 0x03C003C0u) | g.x16), d, m24d));
-}
-
-template <class T>
-__device__ __forceinline__ float4 q4(const T *p);
-template <>
-__device__ __forceinline__ float4 q4<float>(const float *p) {
-  return __ldg(reinterpret_cast<const float4 *>(p));
-}
-template <>
-__device__ __forceinline__ float4 q4<__half>(const __half *p) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-  const float2 a = __half22float2(bits2h(u.x)), b = __half22float2(bits2h(u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 q4<__nv_bfloat16>(const __nv_bfloat16 *p) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xFFFF0000u));
-}
-__device__ __forceinline__ void put4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
-__device__ __forceinline__ void put4(__half *p, float4 v) {
-  *reinterpret_cast<uint2 *>(p) = make_uint2(h2bits(__floats2half2_rn(v.x, v.y)), h2bits(__floats2half2_rn(v.z, v.w)));
-}
-__device__ __forceinline__ void put4(__nv_bfloat16 *p, float4 v) {
-  __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
-}
-
-// One sequence as the call gives it, with lengths that cannot lead outside
-// the buffers; *bad says that they would have.
-struct Seq {
-  uint32_t q0, nq, len;
-};
-__device__ __forceinline__ Seq load_seq(const Kv4AttnParams &p, uint32_t i, bool *bad) {
-  Seq s;
-  s.q0 = p.starts[i];
-  const uint32_t q1 = p.starts[i + 1];
-  s.len = p.kv_lens[i];
-  s.nq = q1 - s.q0;
-  if (q1 < s.q0 || q1 > p.n_rows || s.nq > p.max_q) {
-    s.nq = 0;
-    *bad = true;
-  }
-  const uint64_t most = static_cast<uint64_t>(p.table_width) << p.bt_log2;
-  if (s.len > most) {
-    s.len = static_cast<uint32_t>(most);
-    *bad = true;
-  }
-  return s;
 }
 
 template <class T>
@@ -202,9 +119,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       const uint32_t i = i0 + tid;
       uint64_t w = 0;
       if (i < p.n_seq) {
-        const Seq s = load_seq(p, i, &bad);
+        const Kv4Seq s = kv4_seq(p, i, &bad);
         blind |= s.len < s.nq;
-        w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * ((s.len + kUnit - 1) / kUnit);
+        if (!p.few_only || s.nq * p.group <= kKv4FewRows)
+          w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * ((s.len + kUnit - 1) / kUnit);
       }
       uint64_t inc = w;
 #pragma unroll
@@ -228,7 +146,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     // queries before position 0 see no key and are in no range: zeros
     if (__syncthreads_or(blind) && blockIdx.x == 0)
       for (uint32_t i = 0; i < p.n_seq; ++i) {
-        const Seq s = load_seq(p, i, &bad);
+        const Kv4Seq s = kv4_seq(p, i, &bad);
         const uint32_t cols = p.n_kv * p.group * (kKv4Head / 4);
         const uint64_t n = s.len < s.nq ? static_cast<uint64_t>(s.nq - s.len) * cols : 0;
         for (uint64_t k = tid; k < n; k += 32 * kWarps)
@@ -240,7 +158,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   const uint64_t W = sums[p.n_seq];
   uint64_t G = (W + kMinUnits - 1) / kMinUnits;
   if (G > gridDim.x) G = gridDim.x;
-  if (blockIdx.x >= G) return;
+  if (blockIdx.x >= G) {
+    pdl_wait();
+    return;
+  }
   uint64_t at = W * blockIdx.x / G;
   const uint64_t end = W * (blockIdx.x + 1) / G;
   uint32_t seq = 0;
@@ -260,7 +181,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   while (at < end) {
     while (sums[seq + 1] <= at) ++seq;
     bool bad = false;
-    const Seq s = load_seq(p, seq, &bad);
+    const Kv4Seq s = kv4_seq(p, seq, &bad);
     const uint32_t n_units = (s.len + kUnit - 1) / kUnit;
     const uint32_t pieces = (s.nq * p.group + kRows - 1) / kRows;
     const uint64_t piece = (at - sums[seq]) / n_units;
@@ -583,13 +504,29 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     __syncthreads();       // the merge area and s_last are free again
     at = piece_at + t1;
   }
+  pdl_wait();              // the launch ends no earlier than the one before it
 }
 
 template <class T>
 cudaError_t launch_rows(const Kv4AttnParams &p, int sm_count, cudaStream_t s) {
   const uint32_t smem = kOffSums + (p.n_seq + 1) * 8;
-  kv4_rows_kernel<T><<<sm_count * kCtasPerSm, 32 * kWarps, smem, s>>>(p);
-  return cudaGetLastError();
+  if (!p.few_only) {
+    kv4_rows_kernel<T><<<sm_count * kCtasPerSm, 32 * kWarps, smem, s>>>(p);
+    return cudaGetLastError();
+  }
+  // behind the prompt kernel, which it does not depend on: it may start as
+  // that one's CTAs end, and ends after it
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count * kCtasPerSm);
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_rows_kernel<T>, p);
 }
 
 template <class T>
@@ -598,25 +535,40 @@ cudaError_t rows_setup() {
                               kOffSums + (kKv4MaxSeqs + 1) * 8);
 }
 
+size_t rows_part_floats(int sm_count) { return static_cast<size_t>(sm_count) * kCtasPerSm * 2 * kPartFloats; }
+
 }  // namespace
 
 size_t kv4_attn_part_bytes(int sm_count) {
-  return static_cast<size_t>(sm_count) * kCtasPerSm * 2 * kPartFloats * sizeof(float);
+  return rows_part_floats(sm_count) * sizeof(float) + kv4_prompt_part_bytes(sm_count);
 }
-uint32_t kv4_attn_counters(int sm_count) { return static_cast<uint32_t>(sm_count) * kCtasPerSm; }
+uint32_t kv4_attn_counters(int sm_count) {
+  return static_cast<uint32_t>(sm_count) * kCtasPerSm + kv4_prompt_counters(sm_count);
+}
 
 cudaError_t kv4_attn_setup() {
   cudaError_t e = rows_setup<float>();
   if (e == cudaSuccess) e = rows_setup<__half>();
   if (e == cudaSuccess) e = rows_setup<__nv_bfloat16>();
+  if (e == cudaSuccess) e = kv4_prompt_setup();
   return e;
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnParams &p, Kv4Type t, int sm_count, uint32_t *launches, cudaStream_t s) {
-  cudaError_t e;
-  if (t == KV4_F32) e = launch_rows<float>(p, sm_count, s);
-  else if (t == KV4_F16) e = launch_rows<__half>(p, sm_count, s);
-  else e = launch_rows<__nv_bfloat16>(p, sm_count, s);
+  Kv4AttnParams few = p;
+  few.few_only = static_cast<uint64_t>(p.max_q) * p.group > kKv4FewRows;
+  cudaError_t e = cudaSuccess;
+  if (few.few_only) {
+    Kv4AttnParams many = p;
+    many.part = p.part + rows_part_floats(sm_count);
+    many.counters = p.counters + static_cast<uint32_t>(sm_count) * kCtasPerSm;
+    e = launch_kv4_prompt(many, t, sm_count, s);
+    if (e != cudaSuccess) return e;
+    if (launches) ++*launches;
+  }
+  if (t == KV4_F32) e = launch_rows<float>(few, sm_count, s);
+  else if (t == KV4_F16) e = launch_rows<__half>(few, sm_count, s);
+  else e = launch_rows<__nv_bfloat16>(few, sm_count, s);
   if (e == cudaSuccess && launches) ++*launches;
   return e;
 }

@@ -1,0 +1,755 @@
+// kv4_prompt.cu — attention of prompts and prompt chunks over the paged 4-bit
+// KV cache, on tcgen05.
+//
+// The same formula as kv4_attn.cu for sequences with more than 16 query rows
+// per kv head.  Bound by the tensor cores (4 * 128 flops per query head and
+// key, twice that for f32 rows) and, as closely, by the exponentials: 128 x
+// 128 scores are 1024 cycles of either.
+//
+// A persistent CTA per SM works through pieces (sequence, kv head, row tile);
+// a row tile is 256 query rows of the kv head's group for 16-bit types, 128
+// for f32.  Keys come 128 at a time.  Two streams of softmax run side by
+// side, each 128 rows with its own score columns and accumulator in TMEM, so
+// that one stream's exponentials overlap the other's products:
+//   16-bit rows  stream i is rows 128 i.. of the tile, both see every key tile;
+//   f32 rows     q = hi + lo (binary16 each), S = hi K^T + lo K^T in one
+//                accumulator, P = hi + lo likewise; the streams take the key
+//                tiles in turn and are joined at the end of the piece.
+// The cache's values are exact in binary16 (kv4.h), so f32 rows keep 22 bits.
+//
+// Warps:
+//   0-7    softmax, a row per thread: the scores' maximum, then exponentials
+//          written back over the scores as the A operand of P V.  For 16-bit
+//          rows the accumulator is rescaled only when a row's maximum has
+//          grown by more than 2^8, with P held times 2^7; for f32 rows at
+//          once, with P times 2^15, which keeps it to 2^-40 of the largest;
+//   8-11   query rows and, tile after tile, keys and values: 4-bit words from
+//          the cache to binary16 operands in shared memory, a key word being
+//          one 16-byte chunk of the canonical layout;
+//   12     one thread issues the MMAs: PV(t), then S(t + 2), in order.
+// TMEM (512 columns): S of stream 0 and 1 at 0 and 128, O at 256 and 384.  P
+// lies on its own scores: 32 score columns become 16 of hi and 16 of lo.
+//
+// The work is cut into equal ranges of key tiles as in kv4_attn.cu; pieces cut
+// by a range boundary leave partials that the last CTA to arrive joins.
+// Every wait is bounded; on an expired one each role stops, the MMA thread
+// waits for its own MMAs, and TMEM is freed.
+#include "kv4_rows.cuh"
+#include "tcgen05.cuh"
+
+namespace zgpu {
+
+namespace {
+
+constexpr uint32_t kSoftWarps = 8, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kConvWarps + 1);
+constexpr uint32_t kKeys = 128;                       // keys of a tile
+constexpr uint32_t kOpBytes = 128 * kKv4Head * 2;     // one operand tile: 128 rows x 128 binary16
+constexpr uint32_t kOffQ = 0, kOffK = 2 * kOpBytes, kOffV = 4 * kOpBytes, kOffTab = 6 * kOpBytes;
+constexpr uint32_t kMaxRows = 256;
+constexpr uint32_t kPartFloats = kMaxRows * (kKv4Head + 2);
+constexpr uint32_t kMinTiles = 2;                     // key tiles a range is worth
+constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemCols = 512;
+// kind::f16: D f32, A and B binary16, both K-major, N = 128, M = 128
+constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+// Operand tiles: [row / 8][16-byte chunk][row % 8][16 bytes]
+constexpr uint32_t kLbo = 128, kSbo = 2048;
+
+struct Bars {
+  uint64_t qfull, qempty, kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], ofull[2], oempty[2], join, drain;
+};
+
+// K's four nibble pairs of a word (bits 0, 4, 8, 12 of each half) as (n - 8) d.
+struct KMagic {
+  uint32_t x1024, x64;
+};
+__device__ __forceinline__ void k_values(uint32_t w, __half2 d, const KMagic &g, uint32_t (&v)[4]) {
+  const uint32_t w8 = w >> 8;
+  const __half2 m1032 = __half2half2(__ushort_as_half(0xE408)), m72 = __half2half2(__ushort_as_half(0xD480));
+  v[0] = h2bits(__hmul2(__hadd2(bits2h((w & 0x000F000Fu) | g.x1024), m1032), d));
+  v[1] = h2bits(__hmul2(__hadd2(bits2h((w & 0x00F000F0u) | g.x64), m72), d));
+  v[2] = h2bits(__hmul2(__hadd2(bits2h((w8 & 0x000F000Fu) | g.x1024), m1032), d));
+  v[3] = h2bits(__hmul2(__hadd2(bits2h((w8 & 0x00F000F0u) | g.x64), m72), d));
+}
+
+// A bounded wait of a whole warp with one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t &bar, uint32_t parity, uint32_t *status) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_addr(&bar), parity, status));
+}
+
+// Walks the pieces of a range; every warp walks for itself.
+struct Piece {
+  uint32_t seq, head, rt;        // what
+  uint32_t t0, t1, n;            // key tiles t0 .. t1 - 1 of n
+  Kv4Seq s;
+  uint64_t at;                   // the piece's start in units of work
+};
+
+template <uint32_t MR>
+struct Walk {
+  const uint64_t *sums;
+  const uint32_t *lens, *nqs, *q0s;
+  uint32_t n_kv, group;
+  uint64_t at, end;
+  Piece p;
+  uint32_t n_rt;
+  bool fresh;
+
+  __device__ __forceinline__ static uint32_t row_tiles(uint32_t nq, uint32_t group) { return (nq * group + MR - 1) / MR; }
+  // key tiles that row tile rt sees
+  __device__ __forceinline__ static uint32_t tiles(uint32_t len, uint32_t nq, uint32_t group, uint32_t rt) {
+    const uint32_t toks = min(nq, ((rt + 1) * MR - 1) / group + 1);    // tokens up to the tile's last row's
+    const int64_t see = static_cast<int64_t>(len) - nq + toks;
+    return see > 0 ? static_cast<uint32_t>((see + kKeys - 1) / kKeys) : 0u;
+  }
+  __device__ __forceinline__ void load() {
+    p.s.len = lens[p.seq];
+    p.s.nq = nqs[p.seq];
+    p.s.q0 = q0s[p.seq];
+    n_rt = row_tiles(p.s.nq, group);
+  }
+  // The first piece: all lanes of the warp take part.
+  __device__ __forceinline__ void start(uint32_t n_seq) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, hi = n_seq;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (sums[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    while (sums[lo + 1] <= at) ++lo;
+    p.seq = lo;
+    load();
+    const uint64_t per_head = (sums[lo + 1] - sums[lo]) / n_kv, off = at - sums[lo];
+    p.head = static_cast<uint32_t>(off / per_head);
+    uint64_t rem = off % per_head;
+    for (uint32_t r0 = 0; r0 < n_rt; r0 += 32) {
+      const uint32_t mine = r0 + lane < n_rt ? tiles(p.s.len, p.s.nq, group, r0 + lane) : 0u;
+      uint32_t inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += u;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, rem < inc);
+      if (hit) {
+        const uint32_t l = __ffs(hit) - 1;
+        p.rt = r0 + l;
+        p.n = __shfl_sync(0xffffffffu, mine, l);
+        p.t0 = static_cast<uint32_t>(rem) - (__shfl_sync(0xffffffffu, inc, l) - p.n);
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    fresh = true;
+  }
+  // The next piece of the range, or false.
+  __device__ __forceinline__ bool next() {
+    if (at >= end) return false;
+    if (!fresh) {
+      p.t0 = 0;
+      while (true) {
+        if (++p.rt == n_rt) {
+          p.rt = 0;
+          if (++p.head == n_kv) {
+            p.head = 0;
+            do ++p.seq;
+            while (sums[p.seq + 1] <= at);
+            load();
+          }
+        }
+        p.n = tiles(p.s.len, p.s.nq, group, p.rt);
+        if (p.n) break;
+      }
+    }
+    fresh = false;
+    p.at = at - p.t0;
+    const uint64_t left = end - at;
+    p.t1 = left < p.n - p.t0 ? p.t0 + static_cast<uint32_t>(left) : p.n;
+    at += p.t1 - p.t0;
+    return true;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnParams p) {
+  constexpr bool kLo = sizeof(T) == 4;
+  constexpr uint32_t MR = kLo ? 128 : 256;
+  // P is held times 2^kPShift, and the accumulator is left alone until a
+  // maximum has grown by kLazy: their sum keeps P below 2^15
+  constexpr float kPShift = kLo ? 15.f : 7.f, kLazy = kLo ? 0.f : 8.f;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) Bars bars;
+  __shared__ uint32_t tmem_base, s_last;
+  __shared__ uint64_t s_scan[kThreads / 32];
+  __shared__ float s_scl[kMaxRows];
+  __shared__ float s_ml[2][2][128][2];
+  __shared__ __align__(8) uint8_t s_bad[4][8];                 // 16-key tiles of a key tile that are not in the pool
+  __shared__ __align__(8) uint32_t s_magic[4];
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffTab);
+  uint32_t *lens = reinterpret_cast<uint32_t *>(sums + p.n_seq + 1), *nqs = lens + p.n_seq, *q0s = nqs + p.n_seq;
+
+  // the few-rows kernel behind this one reads nothing that this one writes
+  pdl_launch_dependents();
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    mbar_init(smem_addr(&bars.qfull), kConvWarps);
+    mbar_init(smem_addr(&bars.qempty), 1 + kSoftWarps);     // the last S, and every reader of s_scl
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&bars.kfull[i]), kConvWarps);
+      mbar_init(smem_addr(&bars.kempty[i]), 1);
+      mbar_init(smem_addr(&bars.vfull[i]), kConvWarps);
+      mbar_init(smem_addr(&bars.vempty[i]), 1);
+      mbar_init(smem_addr(&bars.sfull[i]), 1);
+      mbar_init(smem_addr(&bars.pfull[i]), kSoftWarps / 2);
+      mbar_init(smem_addr(&bars.ofull[i]), 1);
+      mbar_init(smem_addr(&bars.oempty[i]), kLo ? kSoftWarps : kSoftWarps / 2);
+    }
+    mbar_init(smem_addr(&bars.join), kSoftWarps);
+    mbar_init(smem_addr(&bars.drain), 1);
+    fence_barrier_init();
+  }
+  // lengths, then the work of each sequence (a warp each), then its sums
+  for (uint32_t i = tid; i < p.n_seq; i += kThreads) {
+    bool bad = false;                     // recorded by the few-rows kernel
+    const Kv4Seq s = kv4_seq(p, i, &bad);
+    lens[i] = s.len;
+    nqs[i] = s.nq * p.group > kKv4FewRows ? s.nq : 0u;
+    q0s[i] = s.q0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  for (uint32_t i = warp; i < p.n_seq; i += kThreads / 32) {
+    const uint32_t nq = nqs[i], n_rt = Walk<MR>::row_tiles(nq, p.group);
+    uint64_t w = 0;
+    for (uint32_t r = lane; r < n_rt; r += 32) w += Walk<MR>::tiles(lens[i], nq, p.group, r);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (lane == 0) sums[i + 1] = w * p.n_kv;
+  }
+  if (tid == 0) sums[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    uint64_t carry = 0;
+    for (uint32_t i0 = 0; i0 < p.n_seq; i0 += 32) {
+      uint64_t inc = i0 + lane < p.n_seq ? sums[i0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += u;
+      }
+      if (i0 + lane < p.n_seq) sums[i0 + lane + 1] = carry + inc;
+      carry += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = tmem_base;
+  const uint64_t W = sums[p.n_seq];
+  uint64_t G = (W + kMinTiles - 1) / kMinTiles;
+  if (G > gridDim.x) G = gridDim.x;
+
+  if (blockIdx.x < G) {
+    Walk<MR> walk;
+    walk.sums = sums, walk.lens = lens, walk.nqs = nqs, walk.q0s = q0s;
+    walk.n_kv = p.n_kv, walk.group = p.group;
+    walk.at = W * blockIdx.x / G;
+    walk.end = W * (blockIdx.x + 1) / G;
+    walk.start(p.n_seq);
+    // steps of a piece with key tiles 0 .. n - 1: stream t & 1, key tile kv_of(t)
+    auto steps = [](uint32_t n) { return kLo ? n : 2 * n; };
+    bool ok = true;
+
+    if (warp >= kSoftWarps + kConvWarps) {
+      // ------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        uint32_t item = 0, kc0 = 0, sp[2] = {0, 0}, oc[2] = {0, 0};
+        const uint32_t q_op = smem_addr(smem) + kOffQ, k_op = smem_addr(smem) + kOffK, v_op = smem_addr(smem) + kOffV;
+        while (ok && walk.next()) {
+          const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
+          ok = mbar_wait(smem_addr(&bars.qfull), item & 1, p.status);
+          if (!ok) break;
+          auto do_s = [&](uint32_t t) -> bool {
+            const uint32_t i = t & 1, kv = kLo ? t : t >> 1, kc = kc0 + kv, stage = kc & 1;
+            if ((kLo || i == 0) && !mbar_wait(smem_addr(&bars.kfull[stage]), (kc >> 1) & 1, p.status)) return false;
+            tc_fence_after();
+            const uint32_t b = k_op + stage * kOpBytes;
+#pragma unroll
+            for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part) {
+              const uint32_t a = q_op + (kLo ? part : i) * kOpBytes;
+#pragma unroll
+              for (uint32_t kk = 0; kk < 8; ++kk)
+                umma_f16_ss(tmem + kTmemS + 128 * i, umma_desc(a + 256 * kk, kLbo, kSbo), umma_desc(b + 256 * kk, kLbo, kSbo),
+                            kIdesc, part || kk);
+            }
+            umma_commit(smem_addr(&bars.sfull[i]));
+            if (kLo || i == 1) umma_commit(smem_addr(&bars.kempty[stage]));
+            if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
+            return true;
+          };
+          ok = do_s(0) && (n_steps < 2 || do_s(1));
+          for (uint32_t t = 0; ok && t < n_steps; ++t) {
+            const uint32_t i = t & 1, kv = kLo ? t : t >> 1, kc = kc0 + kv, stage = kc & 1;
+            ok = mbar_wait(smem_addr(&bars.pfull[i]), sp[i] & 1, p.status);
+            ++sp[i];
+            if (ok && (kLo || i == 0)) ok = mbar_wait(smem_addr(&bars.vfull[stage]), (kc >> 1) & 1, p.status);
+            if (ok && t < 2 && oc[i] > 0) ok = mbar_wait(smem_addr(&bars.oempty[i]), (oc[i] - 1) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t b = v_op + stage * kOpBytes;
+#pragma unroll
+            for (uint32_t kk = 0; kk < 8; ++kk)
+#pragma unroll
+              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
+                umma_f16_ts(tmem + kTmemO + 128 * i, tmem + kTmemS + 128 * i + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part,
+                            umma_desc(b + 256 * kk, kLbo, kSbo), kIdesc, t >= 2 || kk || part);
+            if (kLo || i == 1) umma_commit(smem_addr(&bars.vempty[stage]));
+            if (t + 2 >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
+            if (t + 2 < n_steps) ok = do_s(t + 2);
+          }
+          ++oc[0];
+          if (n_steps > 1) ++oc[1];
+          kc0 += n;
+          ++item;
+        }
+        // every MMA of this thread has completed before TMEM is freed
+        umma_commit(smem_addr(&bars.drain));
+        mbar_wait(smem_addr(&bars.drain), 0, p.status);
+      }
+    } else if (warp >= kSoftWarps) {
+      // ------------------------------- queries, keys and values to binary16
+      const uint32_t cw = warp - kSoftWarps, r = lane >> 2, c = lane & 3;
+      const Magic mg = magic(smem_addr(s_magic));
+      KMagic kg;
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_addr(s_magic + 2)), "r"(0x64006400u), "r"(0x54005400u) : "memory");
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kg.x1024), "=r"(kg.x64) : "r"(smem_addr(s_magic + 2)) : "memory");
+      const uint32_t tpb_log2 = p.bt_log2 - 4;
+      uint32_t item = 0, kc = 0;
+      while (ok && walk.next()) {
+        const Piece &pc = walk.p;
+        const uint32_t n_rows = pc.s.nq * p.group;
+        const uint32_t *table = p.table + static_cast<size_t>(pc.seq) * p.table_width;
+        // this warp's sixteen keys of each half of a key tile: 16 (4 h + cw) ..
+        auto entry = [&](uint32_t t, uint32_t h) -> uint32_t {
+          const uint32_t tile = 8 * t + 4 * h + cw;
+          return t < pc.t1 && tile * kKv4Tile < pc.s.len ? __ldg(table + (tile >> tpb_log2)) : kKv4NoSlot;
+        };
+        // where they lie; keys that are not there are read from block 0, for
+        // the mask to drop
+        const uint8_t *src[2];
+        bool bad[2];
+        auto find = [&](uint32_t t) {
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t tile = 8 * t + 4 * h + cw, block = entry(t, h);
+            const bool there = block < p.n_blocks;
+            bad[h] = !there && t < pc.t1 && tile * kKv4Tile < pc.s.len;
+            src[h] = p.pool + (((static_cast<size_t>(there ? block : 0u) * p.n_kv + pc.head) << tpb_log2) +
+                               (tile & ((1u << tpb_log2) - 1u))) * kKv4TileBytes;
+          }
+        };
+        uint4 kw[2][2], ks[2][2], vw[2][2], vs[2][2];
+        auto fetch_k = [&]() {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              kw[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + 512 * u + 16 * lane));
+              ks[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4Ks + 64 * u + 16 * (r >> 1)));
+            }
+        };
+        auto fetch_v = [&]() {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              vw[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4V + 512 * u + 16 * lane));
+              vs[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4Vs + 64 * u + 16 * c));
+            }
+        };
+        find(pc.t0);
+        if (item > 0) ok = warp_wait(bars.qempty, (item - 1) & 1, p.status);
+        if (!ok) break;
+        // eight rows at a time: lane (r, c) has chunks c, c + 4, c + 8, c + 12 of row r
+        for (uint32_t g = cw; g < MR / 8; g += kConvWarps) {
+          const uint32_t row = pc.rt * MR + 8 * g + r;
+          float4 x[8];
+          float amax = 0.f;
+          const uint32_t tok = row / p.group, hd = row % p.group;
+          const T *qp = static_cast<const T *>(p.q) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.q_stride +
+                        (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head + 8 * c;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            x[k] = row < n_rows ? q4(qp + 32 * (k >> 1) + 4 * (k & 1)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            amax = fmaxf(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))), amax);
+          }
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+          e = e < -100 ? -100 : e > 110 ? 110 : e;
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          if (c == 0)
+            s_scl[8 * g + r] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          uint8_t *dst = smem + kOffQ + kSbo * g + 16 * r;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 y = make_float4(x[2 * k + h].x * down, x[2 * k + h].y * down, x[2 * k + h].z * down, x[2 * k + h].w * down);
+              const __half2 a = __floats2half2_rn(y.x, y.y), b = __floats2half2_rn(y.z, y.w);
+              hi[2 * h] = h2bits(a);
+              hi[2 * h + 1] = h2bits(b);
+              if (kLo) {
+                const float2 fa = __half22float2(a), fb = __half22float2(b);
+                lo[2 * h] = h2bits(__floats2half2_rn(y.x - fa.x, y.y - fa.y));
+                lo[2 * h + 1] = h2bits(__floats2half2_rn(y.z - fb.x, y.w - fb.y));
+              }
+            }
+            *reinterpret_cast<uint4 *>(dst + kLbo * (c + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (c + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
+
+        // words are loaded as the registers of the tile before become free
+        fetch_k();
+        fetch_v();
+        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++kc) {
+          const uint32_t stage = kc & 1;
+          if (kc >= 2) ok = warp_wait(bars.kempty[stage], ((kc >> 1) - 1) & 1, p.status);
+          if (!ok) break;
+          if (lane < 2) {
+            const bool b = lane ? bad[1] : bad[0];
+            s_bad[kc & 3][4 * lane + cw] = b;
+            if (b) atomicOr(p.status, ZDEV_ERR_BOUNDS);
+          }
+          // keys: row = key 64 h + 16 cw + 8 u + r, chunk 4 g + c
+          uint8_t *kd = smem + kOffK + stage * kOpBytes + kSbo * (2 * cw) + 16 * r + kLbo * c;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t w[4] = {kw[h][u].x, kw[h][u].y, kw[h][u].z, kw[h][u].w};
+              const uint32_t s4[4] = {ks[h][u].x, ks[h][u].y, ks[h][u].z, ks[h][u].w};
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const __half2 dd = bits2h(s4[g]);
+                const __half2 d = r & 1 ? __high2half2(dd) : __low2half2(dd);
+                uint32_t v[4];
+                k_values(w[g], d, kg, v);
+                *reinterpret_cast<uint4 *>(kd + kSbo * (8 * h + u) + kLbo * 4 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bars.kfull[stage]));
+          if (t + 1 < pc.t1) {
+            find(t + 1);
+            fetch_k();
+          }
+          // values, transposed: row = dim 32 g + 8 s + r, keys 64 h + 16 cw + 8 u + 2 c and + 1
+          if (kc >= 2) ok = warp_wait(bars.vempty[stage], ((kc >> 1) - 1) & 1, p.status);
+          if (!ok) break;
+          uint8_t *vd = smem + kOffV + stage * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t w[4] = {vw[h][u].x, vw[h][u].y, vw[h][u].z, vw[h][u].w};
+              const uint32_t s4[4] = {vs[h][u].x, vs[h][u].y, vs[h][u].z, vs[h][u].w};
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const __half2 d = bits2h(s4[g]);
+                uint32_t v[4];
+                v_values(w[g], d, __hmul2(d, __float2half2_rn(-24.f)), mg, v);
+#pragma unroll
+                for (int s2 = 0; s2 < 4; ++s2)
+                  *reinterpret_cast<uint32_t *>(vd + kLbo * (8 * h + u) + kSbo * (4 * g + s2)) = v[s2];
+              }
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bars.vfull[stage]));
+          if (t + 1 < pc.t1) fetch_v();
+        }
+        ++item;
+      }
+    } else {
+      // ------------------------------------------------------------ softmax
+      const uint32_t i = warp >> 2, row = 32 * (warp & 3) + lane;     // stream, row of the stream
+      const uint32_t lane_base = tmem + ((32u * (warp & 3)) << 16);
+      const uint32_t s_col = lane_base + kTmemS + 128 * i, o_col = lane_base + kTmemO;
+      uint32_t item = 0, kc0 = 0, ns = 0, oc[2] = {0, 0}, joins = 0;
+      // all softmax warps, with a bounded wait
+      auto join = [&]() -> bool {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bars.join));
+        return warp_wait(bars.join, joins++ & 1, p.status);
+      };
+      while (ok && walk.next()) {
+        const Piece &pc = walk.p;
+        const uint32_t n = pc.t1 - pc.t0, n_steps = steps(n), trow = kLo ? row : 128 * i + row;
+        const uint32_t grow = pc.rt * MR + trow, n_rows = pc.s.nq * p.group;
+        const uint32_t tok = grow / p.group;
+        // keys that the row sees; a row behind the last is for no use
+        const int64_t pos1 = static_cast<int64_t>(pc.s.len) - pc.s.nq + tok + 1;
+        const uint32_t limit = grow >= n_rows ? pc.s.len : pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
+        uint32_t all_see = limit;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
+        ok = warp_wait(bars.qfull, item & 1, p.status);
+        if (!ok) break;
+        const float scl = s_scl[trow];
+        // the next piece's queries wait for this: a piece of one key tile
+        // would otherwise let them run two phases of qfull ahead
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bars.qempty));
+        float m = -INFINITY;
+        float2 l = make_float2(0.f, 0.f);
+        for (uint32_t t = i; ok && t < n_steps; t += 2) {
+          const uint32_t kv = kLo ? t : t >> 1, key0 = (pc.t0 + kv) * kKeys;
+          ok = warp_wait(bars.sfull[i], ns & 1, p.status);
+          ++ns;
+          if (!ok) break;
+          tc_fence_after();
+          const uint2 bad8 = *reinterpret_cast<const uint2 *>(s_bad[(kc0 + kv) & 3]);
+          const bool masked = key0 + kKeys > all_see || (bad8.x | bad8.y);
+          // 32 scores at column c0; a key that the row does not see is -inf
+          auto mask = [&](uint32_t c0, uint32_t (&v)[32]) {
+            const uint64_t bad = bad8.x | static_cast<uint64_t>(bad8.y) << 32;
+#pragma unroll
+            for (uint32_t x = 0; x < 32; ++x)
+              if (key0 + c0 + x >= limit || ((bad >> (8 * ((c0 + x) / 16))) & 1u)) v[x] = 0xFF800000u;
+          };
+          float mx = -INFINITY;
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            tmem_ld32(s_col + 32 * q, v);
+            tmem_ld_wait32(v);
+            if (masked) mask(32 * q, v);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) mx = fmaxf(mx, __uint_as_float(v[x]));
+          }
+          mx *= scl;
+          if (t < 2) {
+            m = mx;
+          } else if (__any_sync(0xffffffffu, mx > m + kLazy)) {
+            // S(t) was issued after PV(t - 2): the accumulator is at rest
+            const float nm = mx > m + kLazy ? mx : m, a = nm == m ? 1.f : ex2(m - nm);
+            l = mul2_rn(l, make_float2(a, a));
+            m = nm;
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+              uint32_t v[32];
+              tmem_ld32(o_col + 128 * i + 32 * q, v);
+              tmem_ld_wait32(v);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * a);
+              tmem_st32(o_col + 128 * i + 32 * q, v);
+            }
+          }
+          const float sub = m == -INFINITY ? kPShift : kPShift - m;
+          const float2 scl2 = make_float2(scl, scl), sub2 = make_float2(sub, sub);
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            tmem_ld32(s_col + 32 * q, v);
+            tmem_ld_wait32(v);
+            if (masked) mask(32 * q, v);
+            uint32_t pk[32];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float2 a = fma2_rn(make_float2(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), scl2, sub2);
+              const float2 e = make_float2(ex2(a.x), ex2(a.y));
+              l = add2_rn(l, e);
+              const __half2 hi = __floats2half2_rn(e.x, e.y);
+              pk[x] = h2bits(hi);
+              if (kLo) {
+                const float2 lo = sub2_rn(e, __half22float2(hi));
+                pk[16 + x] = h2bits(__floats2half2_rn(lo.x, lo.y));
+              }
+            }
+            if (kLo) {
+              tmem_st32(s_col + 32 * q, pk);
+            } else {
+              uint32_t half[16];
+#pragma unroll
+              for (int x = 0; x < 16; ++x) half[x] = pk[x];
+              tmem_st16(s_col + 32 * q, half);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bars.pfull[i]));
+        }
+        // ------------------------------------------ the piece's accumulator
+        const bool use1 = n_steps > 1;
+        if (ok && (kLo || i == 0)) ok = warp_wait(bars.ofull[0], oc[0] & 1, p.status);
+        if (ok && (kLo ? use1 : i == 1)) ok = warp_wait(bars.ofull[1], oc[1] & 1, p.status);
+        ++oc[0];
+        if (use1) ++oc[1];
+        if (!ok) break;
+        tc_fence_after();
+        float M = m, L = l.x + l.y, w0 = 1.f, w1 = 0.f;
+        if (kLo) {
+          // the streams' states of a row: both halves of the warps need both
+          float(*ml)[128][2] = s_ml[item & 1];
+          ml[i][row][0] = M;
+          ml[i][row][1] = L;
+          if (!(ok = join())) break;
+          const float m0 = ml[0][row][0], m1 = ml[1][row][0];
+          M = fmaxf(m0, m1);
+          w0 = m0 == M ? 1.f : ex2(m0 - M);
+          w1 = m1 == M ? 1.f : ex2(m1 - M);
+          L = ml[0][row][1] * w0 + ml[1][row][1] * w1;
+        }
+        const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
+        const bool blind = limit == 0 || grow >= n_rows;
+        const float inv = whole ? 1.f / L : 1.f;
+        if (whole && !blind && !(M == -INFINITY && L == 0.f) && !(L > 0.f && L < INFINITY && fabsf(M) < INFINITY))
+          atomicOr(p.status, ZDEV_ERR_NUMERICAL);
+        T *orow = static_cast<T *>(p.out) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.out_stride +
+                  (static_cast<size_t>(pc.head) * p.group + grow % p.group) * kKv4Head;
+        const bool none = M == -INFINITY && L == 0.f;
+        float *part = p.part + (2ull * blockIdx.x + (pc.t0 == 0 ? 1 : 0)) * kPartFloats;
+        // 32 dims at a time: f32 rows share the row's dims between the streams' warps
+#pragma unroll 1
+        for (uint32_t q = kLo ? 2 * i : 0; q < (kLo ? 2 * i + 2 : 4u); ++q) {
+          uint32_t v[32];
+          tmem_ld32(o_col + (kLo ? 0 : 128 * i) + 32 * q, v);
+          tmem_ld_wait32(v);
+          float o[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = __uint_as_float(v[x]) * w0;
+          if (kLo && use1) {
+            tmem_ld32(o_col + 128 + 32 * q, v);
+            tmem_ld_wait32(v);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = fmaf(__uint_as_float(v[x]), w1, o[x]);
+          }
+          if (whole) {
+            if (!blind)
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                put4(orow + 32 * q + 4 * x, none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                 : make_float4(o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              *reinterpret_cast<float4 *>(part + 4 * ((8 * q + x) * MR + trow)) =
+                  make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kLo) {
+            mbar_arrive(smem_addr(&bars.oempty[0]));
+            if (use1) mbar_arrive(smem_addr(&bars.oempty[1]));
+          } else {
+            mbar_arrive(smem_addr(&bars.oempty[i]));
+          }
+        }
+        if (!whole) {
+          if (!kLo || i == 0) *reinterpret_cast<float2 *>(part + MR * kKv4Head + 2 * trow) = make_float2(M, L);
+          __threadfence();
+          if (!(ok = join())) break;
+          // the ranges that share the piece
+          const uint32_t c0 = static_cast<uint32_t>(((pc.at + 1) * G - 1) / W);
+          const uint32_t c1 = static_cast<uint32_t>(((pc.at + pc.n) * G - 1) / W);
+          if (tid == 0) {
+            s_last = atomicAdd(&p.counters[c0], 1u) == c1 - c0;
+            if (s_last) p.counters[c0] = 0;
+          }
+          if (!(ok = join())) break;
+          if (s_last) {
+            __threadfence();
+            auto from = [&](uint32_t k) { return p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats; };
+            M = -INFINITY;
+            L = 0.f;
+            for (uint32_t k = c0; k <= c1; ++k) {
+              const float2 x = __ldcg(reinterpret_cast<const float2 *>(from(k) + MR * kKv4Head + 2 * trow));
+              if (x.x == -INFINITY && x.y == 0.f) continue;
+              const float nm = fmaxf(M, x.x);
+              L = (M == nm ? L : L * ex2(M - nm)) + (x.x == nm ? x.y : x.y * ex2(x.x - nm));
+              M = nm;
+            }
+            const bool empty = M == -INFINITY && L == 0.f;
+            if (!blind && !empty && !(L > 0.f && L < INFINITY && fabsf(M) < INFINITY)) atomicOr(p.status, ZDEV_ERR_NUMERICAL);
+            const float li = empty ? 0.f : 1.f / L;
+#pragma unroll 1
+            for (uint32_t d0 = kLo ? 16 * i : 0; d0 < (kLo ? 16 * i + 16 : 32u); d0 += 8) {
+              float4 a[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) a[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+              for (uint32_t k = c0; k <= c1; ++k) {
+                const float *src = from(k);
+                const float2 st = __ldcg(reinterpret_cast<const float2 *>(src + MR * kKv4Head + 2 * trow));
+                const float w = st.x == -INFINITY && st.y == 0.f ? 0.f : st.x == M ? 1.f : ex2(st.x - M);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                  const float4 y = __ldcg(reinterpret_cast<const float4 *>(src + 4 * ((d0 + x) * MR + trow)));
+                  a[x].x += y.x * w, a[x].y += y.y * w, a[x].z += y.z * w, a[x].w += y.w * w;
+                }
+              }
+              if (!blind)
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                  put4(orow + 4 * (d0 + x), make_float4(a[x].x * li, a[x].y * li, a[x].z * li, a[x].w * li));
+            }
+          }
+          if (!(ok = join())) break;      // s_last is free again
+        }
+        kc0 += n;
+        ++item;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <class T>
+cudaError_t launch(const Kv4AttnParams &p, int sm_count, cudaStream_t s) {
+  const uint32_t smem = kOffTab + (p.n_seq + 1) * 8 + p.n_seq * 12;
+  kv4_prompt_kernel<T><<<sm_count, kThreads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+template <class T>
+cudaError_t setup() {
+  return cudaFuncSetAttribute(kv4_prompt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              kOffTab + (kKv4MaxSeqs + 1) * 8 + kKv4MaxSeqs * 12);
+}
+
+}  // namespace
+
+size_t kv4_prompt_part_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 2 * kPartFloats * sizeof(float); }
+uint32_t kv4_prompt_counters(int sm_count) { return static_cast<uint32_t>(sm_count); }
+
+cudaError_t kv4_prompt_setup() {
+  cudaError_t e = setup<float>();
+  if (e == cudaSuccess) e = setup<__half>();
+  if (e == cudaSuccess) e = setup<__nv_bfloat16>();
+  return e;
+}
+
+cudaError_t launch_kv4_prompt(const Kv4AttnParams &p, Kv4Type t, int sm_count, cudaStream_t s) {
+  if (t == KV4_F32) return launch<float>(p, sm_count, s);
+  if (t == KV4_F16) return launch<__half>(p, sm_count, s);
+  return launch<__nv_bfloat16>(p, sm_count, s);
+}
+
+}  // namespace zgpu
