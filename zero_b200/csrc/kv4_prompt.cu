@@ -23,10 +23,12 @@
 //          rows the accumulator is rescaled only when a row's maximum has
 //          grown by more than 2^8, with P held times 2^7; for f32 rows at
 //          once, with P times 2^15, which keeps it to 2^-40 of the largest;
-//   8-11   query rows and, tile after tile, keys and values: 4-bit words from
-//          the cache to binary16 operands in shared memory, a key word being
-//          one 16-byte chunk of the canonical layout;
-//   12     one thread issues the MMAs: PV(t), then S(t + 2), in order.
+//   8-11   keys and values, tile after tile, from 4-bit words to binary16
+//          operands in a ring of three, a key word being one 16-byte chunk of
+//          the canonical layout;
+//   12     one thread issues the MMAs: PV(t), then S(t + 2), in order;
+//   13     bulk copies of the tiles' words, two key tiles ahead;
+//   14-15  the next piece's query rows.
 // TMEM (512 columns): S of stream 0 and 1 at 0 and 128, O at 256 and 384.  P
 // lies on its own scores: 32 score columns become 16 of hi and 16 of lo.
 //
@@ -41,10 +43,15 @@ namespace zgpu {
 
 namespace {
 
-constexpr uint32_t kSoftWarps = 8, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kConvWarps + 1);
+constexpr uint32_t kSoftWarps = 8, kConvWarps = 4, kQWarps = 2, kThreads = 512;
+constexpr uint32_t kConv0 = kSoftWarps, kMmaWarp = kConv0 + kConvWarps, kLoadWarp = kMmaWarp + 1, kQ0 = kLoadWarp + 1;
+static_assert(32 * (kQ0 + kQWarps) == kThreads, "every warp has a role");
 constexpr uint32_t kKeys = 128;                       // keys of a tile
 constexpr uint32_t kOpBytes = 128 * kKv4Head * 2;     // one operand tile: 128 rows x 128 binary16
-constexpr uint32_t kOffQ = 0, kOffK = 2 * kOpBytes, kOffV = 4 * kOpBytes, kOffTab = 6 * kOpBytes;
+constexpr uint32_t kSlots = 3;                        // operand tiles of keys and values, in turn
+constexpr uint32_t kRawBytes = kKeys / kKv4Tile * kKv4TileBytes, kRawStages = 2;
+constexpr uint32_t kOffQ = 0, kOffOp = 2 * kOpBytes, kOffRaw = kOffOp + kSlots * kOpBytes;
+constexpr uint32_t kOffTab = kOffRaw + kRawStages * kRawBytes;
 constexpr uint32_t kMaxRows = 256;
 constexpr uint32_t kPartFloats = kMaxRows * (kKv4Head + 2);
 constexpr uint32_t kMinTiles = 2;                     // key tiles a range is worth
@@ -55,7 +62,8 @@ constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24
 constexpr uint32_t kLbo = 128, kSbo = 2048;
 
 struct Bars {
-  uint64_t qfull, qempty, kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], ofull[2], oempty[2], join, drain;
+  uint64_t qfull, qempty, rfull[kRawStages], rempty[kRawStages], full[kSlots], empty[kSlots];
+  uint64_t sfull[2], pfull[2], ofull[2], oempty[2], join, drain;
 };
 
 // K's four nibble pairs of a word (bits 0, 4, 8, 12 of each half) as (n - 8) d.
@@ -71,9 +79,58 @@ __device__ __forceinline__ void k_values(uint32_t w, __half2 d, const KMagic &g,
   v[3] = h2bits(__hmul2(__hadd2(bits2h((w8 & 0x00F000F0u) | g.x64), m72), d));
 }
 
+// Two 16-bit values of a row as f32.
+template <class T>
+__device__ __forceinline__ float2 pair_of(uint32_t u) {
+  if (sizeof(T) == 2 && __is_same(T, __half)) return __half22float2(bits2h(u));
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+
+// 32 bytes to a 32-byte boundary: a whole sector a lane.
+__device__ __forceinline__ void st_sector(void *p, const uint32_t *v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// 32 values of a row.  A lane writes its own row, so a store is worth as many
+// bytes as it can carry: whole sectors where the rows allow it.
+template <class T>
+__device__ __forceinline__ void put32(T *p, const float (&o)[32], bool sectors) {
+  constexpr int kWords = 8 * sizeof(T);
+  uint32_t w[kWords];
+#pragma unroll
+  for (int x = 0; x < kWords; ++x) {
+    if (sizeof(T) == 4) {
+      w[x] = __float_as_uint(o[x]);
+    } else if (__is_same(T, __half)) {
+      w[x] = h2bits(__floats2half2_rn(o[(2 * x) & 31], o[(2 * x + 1) & 31]));
+    } else {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(o[(2 * x) & 31], o[(2 * x + 1) & 31]);
+      w[x] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+  }
+  uint32_t *d = reinterpret_cast<uint32_t *>(p);
+  if (sectors) {
+#pragma unroll
+    for (int x = 0; x < kWords; x += 8) st_sector(d + x, w + x);
+  } else {
+#pragma unroll
+    for (int x = 0; x < kWords; x += 4) *reinterpret_cast<uint4 *>(d + x) = make_uint4(w[x], w[x + 1], w[x + 2], w[x + 3]);
+  }
+}
+
+// Waits with the polling loop out of line: six roles share the instruction
+// cache, and their loops have to stay small (with everything unrolled and
+// inlined the kernel spent more time fetching instructions than issuing them).
+__device__ __noinline__ bool slow_wait(uint32_t bar, uint32_t parity, uint32_t *status) {
+  return mbar_wait(bar, parity, status);
+}
+__device__ __forceinline__ bool wait(uint64_t &bar, uint32_t parity, uint32_t *status) {
+  return mbar_try_wait(smem_addr(&bar), parity) || slow_wait(smem_addr(&bar), parity, status);
+}
 // A bounded wait of a whole warp with one answer for all lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t &bar, uint32_t parity, uint32_t *status) {
-  return __all_sync(0xffffffffu, mbar_wait(smem_addr(&bar), parity, status));
+  return __all_sync(0xffffffffu, wait(bar, parity, status));
 }
 
 // Walks the pieces of a range; every warp walks for itself.
@@ -108,7 +165,7 @@ struct Walk {
     n_rt = row_tiles(p.s.nq, group);
   }
   // The first piece: all lanes of the warp take part.
-  __device__ __forceinline__ void start(uint32_t n_seq) {
+  __device__ __noinline__ void start(uint32_t n_seq) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t lo = 0, hi = n_seq;
     while (hi - lo > 1) {
@@ -143,7 +200,7 @@ struct Walk {
     fresh = true;
   }
   // The next piece of the range, or false.
-  __device__ __forceinline__ bool next() {
+  __device__ __noinline__ bool next() {
     if (at >= end) return false;
     if (!fresh) {
       p.t0 = 0;
@@ -180,10 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) Bars bars;
   __shared__ uint32_t tmem_base, s_last;
-  __shared__ uint64_t s_scan[kThreads / 32];
   __shared__ float s_scl[kMaxRows];
   __shared__ float s_ml[2][2][128][2];
-  __shared__ __align__(8) uint8_t s_bad[4][8];                 // 16-key tiles of a key tile that are not in the pool
+  __shared__ __align__(8) uint8_t s_bad[8][8];                 // 16-key tiles of a key tile that are not in the pool
   __shared__ __align__(8) uint32_t s_magic[4];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffTab);
@@ -198,17 +254,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
-    mbar_init(smem_addr(&bars.qfull), kConvWarps);
+    mbar_init(smem_addr(&bars.qfull), kQWarps);
     mbar_init(smem_addr(&bars.qempty), 1 + kSoftWarps);     // the last S, and every reader of s_scl
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&bars.kfull[i]), kConvWarps);
-      mbar_init(smem_addr(&bars.kempty[i]), 1);
-      mbar_init(smem_addr(&bars.vfull[i]), kConvWarps);
-      mbar_init(smem_addr(&bars.vempty[i]), 1);
       mbar_init(smem_addr(&bars.sfull[i]), 1);
       mbar_init(smem_addr(&bars.pfull[i]), kSoftWarps / 2);
       mbar_init(smem_addr(&bars.ofull[i]), 1);
       mbar_init(smem_addr(&bars.oempty[i]), kLo ? kSoftWarps : kSoftWarps / 2);
+    }
+    for (uint32_t i = 0; i < kRawStages; ++i) {
+      mbar_init(smem_addr(&bars.rfull[i]), 1);
+      mbar_init(smem_addr(&bars.rempty[i]), kConvWarps);
+    }
+    for (uint32_t i = 0; i < kSlots; ++i) {
+      mbar_init(smem_addr(&bars.full[i]), kConvWarps);
+      mbar_init(smem_addr(&bars.empty[i]), 1);
     }
     mbar_init(smem_addr(&bars.join), kSoftWarps);
     mbar_init(smem_addr(&bars.drain), 1);
@@ -265,52 +325,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     auto steps = [](uint32_t n) { return kLo ? n : 2 * n; };
     bool ok = true;
 
-    if (warp >= kSoftWarps + kConvWarps) {
+    if (warp == kMmaWarp) {
       // ------------------------------------------------------- MMA issuer
       if (lane == 0) {
         uint32_t item = 0, kc0 = 0, sp[2] = {0, 0}, oc[2] = {0, 0};
-        const uint32_t q_op = smem_addr(smem) + kOffQ, k_op = smem_addr(smem) + kOffK, v_op = smem_addr(smem) + kOffV;
+        // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
+        const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
+        const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
+        // operand tile x of the ring: key tile kc is x = 2 kc, its values 2 kc + 1
         while (ok && walk.next()) {
           const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
-          ok = mbar_wait(smem_addr(&bars.qfull), item & 1, p.status);
-          if (!ok) break;
-          auto do_s = [&](uint32_t t) -> bool {
-            const uint32_t i = t & 1, kv = kLo ? t : t >> 1, kc = kc0 + kv, stage = kc & 1;
-            if ((kLo || i == 0) && !mbar_wait(smem_addr(&bars.kfull[stage]), (kc >> 1) & 1, p.status)) return false;
-            tc_fence_after();
-            const uint32_t b = k_op + stage * kOpBytes;
+          ok = wait(bars.qfull, item & 1, p.status);
+          // S(0), S(1), then PV(t - 2) and S(t)
+          for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
+            const uint32_t i = t & 1, d = tmem + kTmemO + 128 * i, sc = tmem + kTmemS + 128 * i;
+            if (t >= 2) {
+              const uint32_t x = 2 * (kc0 + (kLo ? t - 2 : (t - 2) >> 1)) + 1, slot = x % kSlots;
+              if (t - 2 < n_steps) {
+                if (kLo || i == 0) ok = wait(bars.full[slot], (x / kSlots) & 1, p.status);
+                if (ok && t < 4 && oc[i] > 0) ok = wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
+                if (ok) ok = wait(bars.pfull[i], sp[i] & 1, p.status);
+                ++sp[i];
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t b = op_desc + slot * (kOpBytes >> 4);
 #pragma unroll
-            for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part) {
-              const uint32_t a = q_op + (kLo ? part : i) * kOpBytes;
+                for (uint32_t kk = 0; kk < 8; ++kk)
 #pragma unroll
-              for (uint32_t kk = 0; kk < 8; ++kk)
-                umma_f16_ss(tmem + kTmemS + 128 * i, umma_desc(a + 256 * kk, kLbo, kSbo), umma_desc(b + 256 * kk, kLbo, kSbo),
-                            kIdesc, part || kk);
+                  for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
+                    umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part, b + 16 * kk, kIdesc, t >= 4 || kk || part);
+                if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
+                if (t >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
+              }
             }
-            umma_commit(smem_addr(&bars.sfull[i]));
-            if (kLo || i == 1) umma_commit(smem_addr(&bars.kempty[stage]));
-            if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
-            return true;
-          };
-          ok = do_s(0) && (n_steps < 2 || do_s(1));
-          for (uint32_t t = 0; ok && t < n_steps; ++t) {
-            const uint32_t i = t & 1, kv = kLo ? t : t >> 1, kc = kc0 + kv, stage = kc & 1;
-            ok = mbar_wait(smem_addr(&bars.pfull[i]), sp[i] & 1, p.status);
-            ++sp[i];
-            if (ok && (kLo || i == 0)) ok = mbar_wait(smem_addr(&bars.vfull[stage]), (kc >> 1) & 1, p.status);
-            if (ok && t < 2 && oc[i] > 0) ok = mbar_wait(smem_addr(&bars.oempty[i]), (oc[i] - 1) & 1, p.status);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t b = v_op + stage * kOpBytes;
+            if (t < n_steps) {
+              const uint32_t x = 2 * (kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
+              if (kLo || i == 0) ok = wait(bars.full[slot], (x / kSlots) & 1, p.status);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t b = op_desc + slot * (kOpBytes >> 4);
 #pragma unroll
-            for (uint32_t kk = 0; kk < 8; ++kk)
+              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part) {
+                const uint64_t a = q_desc + (kLo ? part : i) * (kOpBytes >> 4);
 #pragma unroll
-              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
-                umma_f16_ts(tmem + kTmemO + 128 * i, tmem + kTmemS + 128 * i + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part,
-                            umma_desc(b + 256 * kk, kLbo, kSbo), kIdesc, t >= 2 || kk || part);
-            if (kLo || i == 1) umma_commit(smem_addr(&bars.vempty[stage]));
-            if (t + 2 >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
-            if (t + 2 < n_steps) ok = do_s(t + 2);
+                for (uint32_t kk = 0; kk < 8; ++kk) umma_f16_ss(sc, a + 16 * kk, b + 16 * kk, kIdesc, part || kk);
+              }
+              umma_commit(smem_addr(&bars.sfull[i]));
+              if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
+              if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
+            }
           }
           ++oc[0];
           if (n_steps > 1) ++oc[1];
@@ -319,152 +382,186 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         }
         // every MMA of this thread has completed before TMEM is freed
         umma_commit(smem_addr(&bars.drain));
-        mbar_wait(smem_addr(&bars.drain), 0, p.status);
+        wait(bars.drain, 0, p.status);
       }
-    } else if (warp >= kSoftWarps) {
-      // ------------------------------- queries, keys and values to binary16
-      const uint32_t cw = warp - kSoftWarps, r = lane >> 2, c = lane & 3;
-      const Magic mg = magic(smem_addr(s_magic));
-      KMagic kg;
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_addr(s_magic + 2)), "r"(0x64006400u), "r"(0x54005400u) : "memory");
-      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kg.x1024), "=r"(kg.x64) : "r"(smem_addr(s_magic + 2)) : "memory");
+    } else if (warp == kLoadWarp) {
+      // ------------------------------------------ the key tiles' 4-bit words
+      // lane h < 8: keys 16 h .. of the tile, table entries a tile ahead
       const uint32_t tpb_log2 = p.bt_log2 - 4;
-      uint32_t item = 0, kc = 0;
+      uint32_t kc = 0;
+      while (ok && walk.next()) {
+        const Piece &pc = walk.p;
+        const uint32_t *table = p.table + static_cast<size_t>(pc.seq) * p.table_width;
+        auto entry = [&](uint32_t t) -> uint32_t {
+          const uint32_t tile = 8 * t + lane;
+          return lane < 8 && t < pc.t1 && tile * kKv4Tile < pc.s.len ? __ldg(table + (tile >> tpb_log2)) : kKv4NoSlot;
+        };
+        uint32_t ent = entry(pc.t0);
+        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++kc) {
+          const uint32_t stage = kc % kRawStages, tile = 8 * t + lane;
+          const bool there = ent < p.n_blocks, bad = lane < 8 && !there && tile * kKv4Tile < pc.s.len;
+          // keys that are not there are read from block 0, for the mask to drop
+          const uint8_t *src = p.pool + (((static_cast<size_t>(there ? ent : 0u) * p.n_kv + pc.head) << tpb_log2) +
+                                         (tile & ((1u << tpb_log2) - 1u))) * kKv4TileBytes;
+          ent = entry(t + 1);
+          if (kc >= kRawStages) ok = warp_wait(bars.rempty[stage], (kc / kRawStages - 1) & 1, p.status);
+          if (!ok) break;
+          if (lane < 8) s_bad[kc & 7][lane] = bad;
+          if (bad) atomicOr(p.status, ZDEV_ERR_BOUNDS);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(smem_addr(&bars.rfull[stage]), kRawBytes);
+          __syncwarp();
+          if (lane < 8)
+            bulk_copy_g2s(smem_addr(smem) + kOffRaw + stage * kRawBytes + lane * kKv4TileBytes, src, kKv4TileBytes,
+                          smem_addr(&bars.rfull[stage]));
+        }
+      }
+      // never leave a copy in flight when the CTA may exit
+      for (uint32_t x = kc > kRawStages ? kc - kRawStages : 0; x < kc; ++x)
+        wait(bars.rfull[x % kRawStages], (x / kRawStages) & 1, p.status);
+    } else if (warp >= kQ0) {
+      // -------------------------------------------------------- query rows
+      // eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
+      // kq + 12 of row kr: the eight lanes of a 16-byte store phase write 128
+      // contiguous bytes.  Batches of eight rows are loaded together, the
+      // first before the wait for the queries' place.
+      constexpr uint32_t kVec = kLo ? 8 : 4, kBatch = kLo ? 2 : 4, kGroups = MR / 8 / kQWarps;
+      const uint32_t qw = warp - kQ0, kr = lane & 7, kq = lane >> 3;
+      uint32_t item = 0;
       while (ok && walk.next()) {
         const Piece &pc = walk.p;
         const uint32_t n_rows = pc.s.nq * p.group;
-        const uint32_t *table = p.table + static_cast<size_t>(pc.seq) * p.table_width;
-        // this warp's sixteen keys of each half of a key tile: 16 (4 h + cw) ..
-        auto entry = [&](uint32_t t, uint32_t h) -> uint32_t {
-          const uint32_t tile = 8 * t + 4 * h + cw;
-          return t < pc.t1 && tile * kKv4Tile < pc.s.len ? __ldg(table + (tile >> tpb_log2)) : kKv4NoSlot;
-        };
-        // where they lie; keys that are not there are read from block 0, for
-        // the mask to drop
-        const uint8_t *src[2];
-        bool bad[2];
-        auto find = [&](uint32_t t) {
+        uint4 raw[kBatch][kVec];
+        auto load_q = [&](uint32_t j0) {
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            const uint32_t tile = 8 * t + 4 * h + cw, block = entry(t, h);
-            const bool there = block < p.n_blocks;
-            bad[h] = !there && t < pc.t1 && tile * kKv4Tile < pc.s.len;
-            src[h] = p.pool + (((static_cast<size_t>(there ? block : 0u) * p.n_kv + pc.head) << tpb_log2) +
-                               (tile & ((1u << tpb_log2) - 1u))) * kKv4TileBytes;
+          for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t row = pc.rt * MR + 8 * (qw + kQWarps * (j0 + j)) + kr, tok = row / p.group, hd = row % p.group;
+            const T *qp = static_cast<const T *>(p.q) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.q_stride +
+                          (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head + 8 * kq;
+#pragma unroll
+            for (uint32_t k = 0; k < kVec; ++k)
+              raw[j][k] = row < n_rows ? __ldg(reinterpret_cast<const uint4 *>(qp + (kLo ? 32 * (k / 2) + 4 * (k & 1) : 32 * k)))
+                                       : make_uint4(0u, 0u, 0u, 0u);
           }
         };
-        uint4 kw[2][2], ks[2][2], vw[2][2], vs[2][2];
-        auto fetch_k = [&]() {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              kw[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + 512 * u + 16 * lane));
-              ks[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4Ks + 64 * u + 16 * (r >> 1)));
-            }
-        };
-        auto fetch_v = [&]() {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              vw[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4V + 512 * u + 16 * lane));
-              vs[h][u] = __ldg(reinterpret_cast<const uint4 *>(src[h] + kKv4Vs + 64 * u + 16 * c));
-            }
-        };
-        find(pc.t0);
+        load_q(0);
         if (item > 0) ok = warp_wait(bars.qempty, (item - 1) & 1, p.status);
         if (!ok) break;
-        // eight rows at a time: lane (r, c) has chunks c, c + 4, c + 8, c + 12 of row r
-        for (uint32_t g = cw; g < MR / 8; g += kConvWarps) {
-          const uint32_t row = pc.rt * MR + 8 * g + r;
-          float4 x[8];
-          float amax = 0.f;
-          const uint32_t tok = row / p.group, hd = row % p.group;
-          const T *qp = static_cast<const T *>(p.q) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.q_stride +
-                        (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head + 8 * c;
+#pragma unroll 1
+        for (uint32_t j0 = 0; j0 < kGroups; j0 += kBatch) {
+          if (j0) load_q(j0);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            x[k] = row < n_rows ? q4(qp + 32 * (k >> 1) + 4 * (k & 1)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            amax = fmaxf(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))), amax);
-          }
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-          e = e < -100 ? -100 : e > 110 ? 110 : e;
-          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          if (c == 0)
-            s_scl[8 * g + r] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          uint8_t *dst = smem + kOffQ + kSbo * g + 16 * r;
+          for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t g = qw + kQWarps * (j0 + j);
+            float amax = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t hi[4], lo[4];
+            for (uint32_t k = 0; k < kVec; ++k) {
+              const uint32_t u[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float4 y = make_float4(x[2 * k + h].x * down, x[2 * k + h].y * down, x[2 * k + h].z * down, x[2 * k + h].w * down);
-              const __half2 a = __floats2half2_rn(y.x, y.y), b = __floats2half2_rn(y.z, y.w);
-              hi[2 * h] = h2bits(a);
-              hi[2 * h + 1] = h2bits(b);
-              if (kLo) {
-                const float2 fa = __half22float2(a), fb = __half22float2(b);
-                lo[2 * h] = h2bits(__floats2half2_rn(y.x - fa.x, y.y - fa.y));
-                lo[2 * h + 1] = h2bits(__floats2half2_rn(y.z - fb.x, y.w - fb.y));
+              for (int x = 0; x < 4; ++x) {
+                if (kLo) {
+                  amax = fmaxf(amax, fabsf(__uint_as_float(u[x])));
+                } else {
+                  const float2 f = pair_of<T>(u[x]);
+                  amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
               }
             }
-            *reinterpret_cast<uint4 *>(dst + kLbo * (c + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (c + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+            int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+            e = e < -100 ? -100 : e > 110 ? 110 : e;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            if (kq == 0)
+              s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            uint8_t *dst = smem + kOffQ + kSbo * g + 16 * kr;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                float2 f;
+                if (kLo) {
+                  const uint4 u = raw[j][kLo ? 2 * k + (x >> 1) : 0];
+                  f = x & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
+                            : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+                } else {
+                  const uint4 u = raw[j][k];
+                  f = pair_of<T>(x == 0 ? u.x : x == 1 ? u.y : x == 2 ? u.z : u.w);
+                }
+                f.x *= down, f.y *= down;
+                const __half2 h = __floats2half2_rn(f.x, f.y);
+                hi[x] = h2bits(h);
+                if (kLo) {
+                  const float2 b = __half22float2(h);
+                  lo[x] = h2bits(__floats2half2_rn(f.x - b.x, f.y - b.y));
+                }
+              }
+              *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (kq + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
-
-        // words are loaded as the registers of the tile before become free
-        fetch_k();
-        fetch_v();
-        for (uint32_t t = pc.t0; t < pc.t1; ++t, ++kc) {
-          const uint32_t stage = kc & 1;
-          if (kc >= 2) ok = warp_wait(bars.kempty[stage], ((kc >> 1) - 1) & 1, p.status);
+        ++item;
+      }
+    } else if (warp >= kConv0) {
+      // --------------------------------------- keys and values to binary16
+      const uint32_t cw = warp - kConv0, r = lane >> 2, c = lane & 3, kr = lane & 7, kq = lane >> 3;
+      const Magic mg = magic(smem_addr(s_magic));
+      KMagic kg;
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_addr(s_magic + 2)), "r"(0x64006400u), "r"(0x54005400u) : "memory");
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kg.x1024), "=r"(kg.x64) : "r"(smem_addr(s_magic + 2)) : "memory");
+      // operand tile x may be written once the MMAs that read tile x - 3 are done
+      auto slot_free = [&](uint32_t x) { return x < kSlots || warp_wait(bars.empty[x % kSlots], (x / kSlots - 1) & 1, p.status); };
+      auto hand_over = [&](uint32_t x) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bars.full[x % kSlots]));
+      };
+      uint32_t kc = 0;
+      while (ok && walk.next()) {
+        const uint32_t n = walk.p.t1 - walk.p.t0;
+        for (uint32_t t = 0; t < n; ++t, ++kc) {
+          const uint32_t stage = kc % kRawStages, x = 2 * kc;
+          ok = warp_wait(bars.rfull[stage], (kc / kRawStages) & 1, p.status) && slot_free(x);
           if (!ok) break;
-          if (lane < 2) {
-            const bool b = lane ? bad[1] : bad[0];
-            s_bad[kc & 3][4 * lane + cw] = b;
-            if (b) atomicOr(p.status, ZDEV_ERR_BOUNDS);
-          }
-          // keys: row = key 64 h + 16 cw + 8 u + r, chunk 4 g + c
-          uint8_t *kd = smem + kOffK + stage * kOpBytes + kSbo * (2 * cw) + 16 * r + kLbo * c;
-#pragma unroll
+          // this warp's sixteen keys of each half of the tile: 16 (4 h + cw) ..
+          const uint8_t *raw = smem + kOffRaw + stage * kRawBytes + cw * kKv4TileBytes;
+          // keys: row = key 64 h + 16 cw + 8 u + kr, chunk 4 g + kq
+          uint8_t *kd = smem + kOffOp + (x % kSlots) * kOpBytes + kSbo * (2 * cw) + 16 * kr + kLbo * kq;
+#pragma unroll 1
           for (int h = 0; h < 2; ++h)
-#pragma unroll
+#pragma unroll 1
             for (int u = 0; u < 2; ++u) {
-              const uint32_t w[4] = {kw[h][u].x, kw[h][u].y, kw[h][u].z, kw[h][u].w};
-              const uint32_t s4[4] = {ks[h][u].x, ks[h][u].y, ks[h][u].z, ks[h][u].w};
+              const uint8_t *src = raw + 4 * h * kKv4TileBytes;
+              const uint4 kw = *reinterpret_cast<const uint4 *>(src + 512 * u + 64 * kr + 16 * kq);
+              const uint4 ks = *reinterpret_cast<const uint4 *>(src + kKv4Ks + 64 * u + 16 * (kr >> 1));
+              const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w}, s4[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 const __half2 dd = bits2h(s4[g]);
-                const __half2 d = r & 1 ? __high2half2(dd) : __low2half2(dd);
+                const __half2 d = kr & 1 ? __high2half2(dd) : __low2half2(dd);
                 uint32_t v[4];
                 k_values(w[g], d, kg, v);
                 *reinterpret_cast<uint4 *>(kd + kSbo * (8 * h + u) + kLbo * 4 * g) = make_uint4(v[0], v[1], v[2], v[3]);
               }
             }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_addr(&bars.kfull[stage]));
-          if (t + 1 < pc.t1) {
-            find(t + 1);
-            fetch_k();
-          }
+          hand_over(x);
           // values, transposed: row = dim 32 g + 8 s + r, keys 64 h + 16 cw + 8 u + 2 c and + 1
-          if (kc >= 2) ok = warp_wait(bars.vempty[stage], ((kc >> 1) - 1) & 1, p.status);
+          ok = slot_free(x + 1);
           if (!ok) break;
-          uint8_t *vd = smem + kOffV + stage * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
-#pragma unroll
+          uint8_t *vd = smem + kOffOp + ((x + 1) % kSlots) * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
+#pragma unroll 1
           for (int h = 0; h < 2; ++h)
-#pragma unroll
+#pragma unroll 1
             for (int u = 0; u < 2; ++u) {
-              const uint32_t w[4] = {vw[h][u].x, vw[h][u].y, vw[h][u].z, vw[h][u].w};
-              const uint32_t s4[4] = {vs[h][u].x, vs[h][u].y, vs[h][u].z, vs[h][u].w};
+              const uint8_t *src = raw + 4 * h * kKv4TileBytes + kKv4V;
+              const uint4 vw = *reinterpret_cast<const uint4 *>(src + 512 * u + 16 * lane);
+              const uint4 vs = *reinterpret_cast<const uint4 *>(src + (kKv4Vs - kKv4V) + 64 * u + 16 * c);
+              const uint32_t w[4] = {vw.x, vw.y, vw.z, vw.w}, s4[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 const __half2 d = bits2h(s4[g]);
@@ -475,12 +572,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
                   *reinterpret_cast<uint32_t *>(vd + kLbo * (8 * h + u) + kSbo * (4 * g + s2)) = v[s2];
               }
             }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_addr(&bars.vfull[stage]));
-          if (t + 1 < pc.t1) fetch_v();
+          hand_over(x + 1);
+          if (lane == 0) mbar_arrive(smem_addr(&bars.rempty[stage]));
         }
-        ++item;
       }
     } else {
       // ------------------------------------------------------------ softmax
@@ -488,6 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       const uint32_t lane_base = tmem + ((32u * (warp & 3)) << 16);
       const uint32_t s_col = lane_base + kTmemS + 128 * i, o_col = lane_base + kTmemO;
       uint32_t item = 0, kc0 = 0, ns = 0, oc[2] = {0, 0}, joins = 0;
+      const bool sectors = ((reinterpret_cast<uintptr_t>(p.out) | p.out_stride * sizeof(T)) & 31u) == 0;
       // all softmax warps, with a bounded wait
       auto join = [&]() -> bool {
         __syncwarp();
@@ -513,79 +608,83 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&bars.qempty));
         float m = -INFINITY;
-        float2 l = make_float2(0.f, 0.f);
+        float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         for (uint32_t t = i; ok && t < n_steps; t += 2) {
           const uint32_t kv = kLo ? t : t >> 1, key0 = (pc.t0 + kv) * kKeys;
           ok = warp_wait(bars.sfull[i], ns & 1, p.status);
           ++ns;
           if (!ok) break;
           tc_fence_after();
-          const uint2 bad8 = *reinterpret_cast<const uint2 *>(s_bad[(kc0 + kv) & 3]);
-          const bool masked = key0 + kKeys > all_see || (bad8.x | bad8.y);
-          // 32 scores at column c0; a key that the row does not see is -inf
-          auto mask = [&](uint32_t c0, uint32_t (&v)[32]) {
+          const uint2 bad8 = *reinterpret_cast<const uint2 *>(s_bad[(kc0 + kv) & 7]);
+          // a key that the row does not see is -inf; written back, so that the
+          // second pass need not ask
+          if (key0 + kKeys > all_see || (bad8.x | bad8.y)) {
             const uint64_t bad = bad8.x | static_cast<uint64_t>(bad8.y) << 32;
+#pragma unroll 1
+            for (uint32_t q = 0; q < 4; ++q) {
+              const uint32_t k0 = key0 + 32 * q, see = limit > k0 ? limit - k0 : 0u;
+              const bool bad0 = (bad >> (16 * q)) & 1u, bad1 = (bad >> (16 * q + 8)) & 1u;
+              uint32_t v[32];
+              tmem_ld32(s_col + 32 * q, v);
+              tmem_ld_wait32(v);
 #pragma unroll
-            for (uint32_t x = 0; x < 32; ++x)
-              if (key0 + c0 + x >= limit || ((bad >> (8 * ((c0 + x) / 16))) & 1u)) v[x] = 0xFF800000u;
-          };
-          float mx = -INFINITY;
-#pragma unroll
-          for (uint32_t q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            tmem_ld32(s_col + 32 * q, v);
-            tmem_ld_wait32(v);
-            if (masked) mask(32 * q, v);
-#pragma unroll
-            for (int x = 0; x < 32; ++x) mx = fmaxf(mx, __uint_as_float(v[x]));
+              for (uint32_t x = 0; x < 32; ++x)
+                if (x >= see || (x < 16 ? bad0 : bad1)) v[x] = 0xFF800000u;
+              tmem_st32(s_col + 32 * q, v);
+            }
+            tmem_st_wait();
           }
-          mx *= scl;
+          // the largest score, in four chains of maxima
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t va[32];
+#pragma unroll 1
+          for (uint32_t q = 0; q < 4; ++q) {
+            tmem_ld32(s_col + 32 * q, va);
+            tmem_ld_wait32(va);
+#pragma unroll
+            for (int x = 0; x < 32; x += 2)
+              mx4[(x >> 1) & 3] = fmaxf(fmaxf(mx4[(x >> 1) & 3], __uint_as_float(va[x])), __uint_as_float(va[x + 1]));
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scl;
           if (t < 2) {
             m = mx;
           } else if (__any_sync(0xffffffffu, mx > m + kLazy)) {
             // S(t) was issued after PV(t - 2): the accumulator is at rest
-            const float nm = mx > m + kLazy ? mx : m, a = nm == m ? 1.f : ex2(m - nm);
-            l = mul2_rn(l, make_float2(a, a));
+            const float nm = mx > m + kLazy ? mx : m, f = nm == m ? 1.f : ex2(m - nm);
+            const float2 ff = make_float2(f, f);
+            l[0] = mul2_rn(l[0], ff), l[1] = mul2_rn(l[1], ff);
             m = nm;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t q = 0; q < 4; ++q) {
-              uint32_t v[32];
-              tmem_ld32(o_col + 128 * i + 32 * q, v);
-              tmem_ld_wait32(v);
+              tmem_ld32(o_col + 128 * i + 32 * q, va);
+              tmem_ld_wait32(va);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * a);
-              tmem_st32(o_col + 128 * i + 32 * q, v);
+              for (int x = 0; x < 32; ++x) va[x] = __float_as_uint(__uint_as_float(va[x]) * f);
+              tmem_st32(o_col + 128 * i + 32 * q, va);
             }
           }
           const float sub = m == -INFINITY ? kPShift : kPShift - m;
           const float2 scl2 = make_float2(scl, scl), sub2 = make_float2(sub, sub);
-#pragma unroll
+          // 32 scores to P in their own columns: 16 of hi, 16 of lo
+#pragma unroll 1
           for (uint32_t q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            tmem_ld32(s_col + 32 * q, v);
-            tmem_ld_wait32(v);
-            if (masked) mask(32 * q, v);
-            uint32_t pk[32];
+            tmem_ld32(s_col + 32 * q, va);
+            tmem_ld_wait32(va);
+            uint32_t hi[16], lo[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-              const float2 a = fma2_rn(make_float2(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), scl2, sub2);
-              const float2 e = make_float2(ex2(a.x), ex2(a.y));
-              l = add2_rn(l, e);
-              const __half2 hi = __floats2half2_rn(e.x, e.y);
-              pk[x] = h2bits(hi);
+              const float2 y = fma2_rn(make_float2(__uint_as_float(va[2 * x]), __uint_as_float(va[2 * x + 1])), scl2, sub2);
+              const float2 e = make_float2(ex2(y.x), ex2(y.y));
+              l[x & 1] = add2_rn(l[x & 1], e);
+              const __half2 h = __floats2half2_rn(e.x, e.y);
+              hi[x] = h2bits(h);
               if (kLo) {
-                const float2 lo = sub2_rn(e, __half22float2(hi));
-                pk[16 + x] = h2bits(__floats2half2_rn(lo.x, lo.y));
+                const float2 d = sub2_rn(e, __half22float2(h));
+                lo[x] = h2bits(__floats2half2_rn(d.x, d.y));
               }
             }
-            if (kLo) {
-              tmem_st32(s_col + 32 * q, pk);
-            } else {
-              uint32_t half[16];
-#pragma unroll
-              for (int x = 0; x < 16; ++x) half[x] = pk[x];
-              tmem_st16(s_col + 32 * q, half);
-            }
+            tmem_st16(s_col + 32 * q, hi);
+            if (kLo) tmem_st16(s_col + 32 * q + 16, lo);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -600,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         if (use1) ++oc[1];
         if (!ok) break;
         tc_fence_after();
-        float M = m, L = l.x + l.y, w0 = 1.f, w1 = 0.f;
+        float M = m, L = (l[0].x + l[0].y) + (l[1].x + l[1].y), w0 = 1.f, w1 = 0.f;
         if (kLo) {
           // the streams' states of a row: both halves of the warps need both
           float(*ml)[128][2] = s_ml[item & 1];
@@ -638,11 +737,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             for (int x = 0; x < 32; ++x) o[x] = fmaf(__uint_as_float(v[x]), w1, o[x]);
           }
           if (whole) {
-            if (!blind)
 #pragma unroll
-              for (int x = 0; x < 8; ++x)
-                put4(orow + 32 * q + 4 * x, none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                 : make_float4(o[4 * x] * inv, o[4 * x + 1] * inv, o[4 * x + 2] * inv, o[4 * x + 3] * inv));
+            for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : o[x] * inv;
+            if (!blind) put32(orow + 32 * q, o, sectors);
           } else {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
