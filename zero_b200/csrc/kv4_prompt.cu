@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
   __shared__ float s_ml[2][2][128][2];
   __shared__ __align__(8) uint8_t s_bad[8][8];                 // 16-key tiles of a key tile that are not in the pool
   __shared__ __align__(8) uint32_t s_magic[4];
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the shuffle makes the roles' branches uniform: the MMA warp's operands
+  // stay in uniform registers
+  const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffTab);
   uint32_t *lens = reinterpret_cast<uint32_t *>(sums + p.n_seq + 1), *nqs = lens + p.n_seq, *q0s = nqs + p.n_seq;
 
@@ -327,63 +329,66 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
 
     if (warp == kMmaWarp) {
       // ------------------------------------------------------- MMA issuer
-      if (lane == 0) {
-        uint32_t item = 0, kc0 = 0, sp[2] = {0, 0}, oc[2] = {0, 0};
-        // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
-        const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
-        const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
-        // operand tile x of the ring: key tile kc is x = 2 kc, its values 2 kc + 1
-        while (ok && walk.next()) {
-          const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
-          ok = wait(bars.qfull, item & 1, p.status);
-          // S(0), S(1), then PV(t - 2) and S(t)
-          for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
-            const uint32_t i = t & 1, d = tmem + kTmemO + 128 * i, sc = tmem + kTmemS + 128 * i;
-            if (t >= 2) {
-              const uint32_t x = 2 * (kc0 + (kLo ? t - 2 : (t - 2) >> 1)) + 1, slot = x % kSlots;
-              if (t - 2 < n_steps) {
-                if (kLo || i == 0) ok = wait(bars.full[slot], (x / kSlots) & 1, p.status);
-                if (ok && t < 4 && oc[i] > 0) ok = wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
-                if (ok) ok = wait(bars.pfull[i], sp[i] & 1, p.status);
-                ++sp[i];
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t b = op_desc + slot * (kOpBytes >> 4);
+      // The whole warp waits and counts; one elected lane issues.
+      uint32_t item = 0, kc0 = 0, sp[2] = {0, 0}, oc[2] = {0, 0};
+      // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
+      const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
+      const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
+      // operand tile x of the ring: key tile kc is x = 2 kc, its values 2 kc + 1
+      while (ok && walk.next()) {
+        const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
+        ok = warp_wait(bars.qfull, item & 1, p.status);
+        // S(0), S(1), then PV(t - 2) and S(t)
+        for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
+          const uint32_t i = t & 1, d = tmem + kTmemO + 128 * i, sc = tmem + kTmemS + 128 * i;
+          if (t >= 2 && t - 2 < n_steps) {
+            const uint32_t x = 2 * (kc0 + (kLo ? t - 2 : (t - 2) >> 1)) + 1, slot = x % kSlots;
+            if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
+            if (ok && t < 4 && oc[i] > 0) ok = warp_wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
+            if (ok) ok = warp_wait(bars.pfull[i], sp[i] & 1, p.status);
+            ++sp[i];
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t b = op_desc + slot * (kOpBytes >> 4);
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < 8; ++kk)
+#pragma unroll
+                for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
+                  umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part, b + 16 * kk, kIdesc, t >= 4 || kk || part);
+              if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
+              if (t >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
+            }
+            __syncwarp();
+          }
+          if (t < n_steps) {
+            const uint32_t x = 2 * (kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
+            if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t b = op_desc + slot * (kOpBytes >> 4), a0 = q_desc + (kLo ? 0 : i) * (kOpBytes >> 4);
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
 #pragma unroll
                 for (uint32_t kk = 0; kk < 8; ++kk)
-#pragma unroll
-                  for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
-                    umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part, b + 16 * kk, kIdesc, t >= 4 || kk || part);
-                if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
-                if (t >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
-              }
-            }
-            if (t < n_steps) {
-              const uint32_t x = 2 * (kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
-              if (kLo || i == 0) ok = wait(bars.full[slot], (x / kSlots) & 1, p.status);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t b = op_desc + slot * (kOpBytes >> 4);
-#pragma unroll
-              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part) {
-                const uint64_t a = q_desc + (kLo ? part : i) * (kOpBytes >> 4);
-#pragma unroll
-                for (uint32_t kk = 0; kk < 8; ++kk) umma_f16_ss(sc, a + 16 * kk, b + 16 * kk, kIdesc, part || kk);
-              }
+                  umma_f16_ss(sc, a0 + part * (kOpBytes >> 4) + 16 * kk, b + 16 * kk, kIdesc, part || kk);
               umma_commit(smem_addr(&bars.sfull[i]));
               if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
               if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
             }
+            __syncwarp();
           }
-          ++oc[0];
-          if (n_steps > 1) ++oc[1];
-          kc0 += n;
-          ++item;
         }
-        // every MMA of this thread has completed before TMEM is freed
-        umma_commit(smem_addr(&bars.drain));
-        wait(bars.drain, 0, p.status);
+        ++oc[0];
+        if (n_steps > 1) ++oc[1];
+        kc0 += n;
+        ++item;
       }
+      // every MMA has completed before TMEM is freed
+      if (elect_one()) umma_commit(smem_addr(&bars.drain));
+      __syncwarp();
+      wait(bars.drain, 0, p.status);
     } else if (warp == kLoadWarp) {
       // ------------------------------------------ the key tiles' 4-bit words
       // lane h < 8: keys 16 h .. of the tile, table entries a tile ahead
