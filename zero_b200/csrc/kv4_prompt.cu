@@ -28,7 +28,7 @@
 //          the canonical layout;
 //   12     one thread issues the MMAs: PV(t), then S(t + 2), in order;
 //   13     bulk copies of the tiles' words, two key tiles ahead;
-//   14-15  the next piece's query rows.
+//   14-15  the next piece's query rows, together with 8-11.
 // TMEM (512 columns): S of stream 0 and 1 at 0 and 128, O at 256 and 384.  P
 // lies on its own scores: 32 score columns become 16 of hi and 16 of lo.
 //
@@ -77,13 +77,6 @@ __device__ __forceinline__ void k_values(uint32_t w, __half2 d, const KMagic &g,
   v[1] = h2bits(__hmul2(__hadd2(bits2h((w & 0x00F000F0u) | g.x64), m72), d));
   v[2] = h2bits(__hmul2(__hadd2(bits2h((w8 & 0x000F000Fu) | g.x1024), m1032), d));
   v[3] = h2bits(__hmul2(__hadd2(bits2h((w8 & 0x00F000F0u) | g.x64), m72), d));
-}
-
-// Two 16-bit values of a row as f32.
-template <class T>
-__device__ __forceinline__ float2 pair_of(uint32_t u) {
-  if (sizeof(T) == 2 && __is_same(T, __half)) return __half22float2(bits2h(u));
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
 
 // 32 bytes to a 32-byte boundary: a whole sector a lane.
@@ -227,6 +220,99 @@ struct Walk {
   }
 };
 
+// One of kConvWarps + kQWarps warps' share of a piece's query rows: binary16
+// (hi and lo for f32) in the operand layout, and each row's factor of the
+// scores.  Eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
+// kq + 12 of row kr: the eight lanes of a 16-byte store phase write 128
+// contiguous bytes.  f32 and bf16 rows are scaled by a power of two (the
+// largest value in [1, 2)) to fit binary16's range; f16 rows are copied.
+template <class T>
+__device__ __noinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
+                                          uint32_t share) {
+  constexpr bool kLo = sizeof(T) == 4, kCopy = __is_same(T, __half);
+  constexpr uint32_t MR = kLo ? 128 : 256, kVec = kLo ? 8 : 4, kBatch = kLo ? 1 : 3, kShares = kConvWarps + kQWarps;
+  const uint32_t lane = threadIdx.x & 31, kr = lane & 7, kq = lane >> 3, n_rows = pc.s.nq * p.group;
+  const uint32_t seq_q0 = pc.s.q0, head = pc.head, row0 = pc.rt * MR;
+#pragma unroll 1
+  for (uint32_t g0 = share; g0 < MR / 8; g0 += kShares * kBatch) {
+    uint4 raw[kBatch][kVec];
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const uint32_t g = g0 + kShares * j, row = row0 + 8 * g + kr, tok = row / p.group, hd = row % p.group;
+      const T *qp = static_cast<const T *>(p.q) + (seq_q0 + static_cast<uint64_t>(tok)) * p.q_stride +
+                    (static_cast<size_t>(head) * p.group + hd) * kKv4Head + 8 * kq;
+#pragma unroll
+      for (uint32_t k = 0; k < kVec; ++k)
+        raw[j][k] = g < MR / 8 && row < n_rows ? __ldg(reinterpret_cast<const uint4 *>(qp + (kLo ? 32 * (k / 2) + 4 * (k & 1) : 32 * k)))
+                                               : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const uint32_t g = g0 + kShares * j;
+      if (g >= MR / 8) break;
+      uint8_t *dst = q_op + kSbo * g + 16 * kr;
+      int e = 0;
+      if (!kCopy) {
+        float amax = 0.f;
+        if (kLo) {
+#pragma unroll
+          for (uint32_t k = 0; k < kVec; ++k)
+            amax = fmaxf(fmaxf(fmaxf(fabsf(__uint_as_float(raw[j][k].x)), fabsf(__uint_as_float(raw[j][k].y))),
+                               fmaxf(fabsf(__uint_as_float(raw[j][k].z)), fabsf(__uint_as_float(raw[j][k].w)))), amax);
+        } else {
+          __nv_bfloat162 mx = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+          for (uint32_t k = 0; k < kVec; ++k) {
+            const uint32_t u[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx = __hmax2(mx, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&u[x])));
+          }
+          amax = fmaxf(__low2float(mx), __high2float(mx));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+        e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+        e = e < -100 ? -100 : e > 110 ? 110 : e;
+      }
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      if (kq == 0)
+        s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (kCopy) {
+          *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = raw[j][k];
+          continue;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float2 f;
+          if (kLo) {
+            const uint4 u = raw[j][kLo ? 2 * k + (x >> 1) : 0];
+            f = x & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
+                      : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+          } else {
+            const uint4 u = raw[j][k];
+            const uint32_t w = x == 0 ? u.x : x == 1 ? u.y : x == 2 ? u.z : u.w;
+            f = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+          }
+          f = mul2_rn(f, make_float2(down, down));
+          const __half2 h = __floats2half2_rn(f.x, f.y);
+          hi[x] = h2bits(h);
+          if (kLo) {
+            const float2 b = __half22float2(h);
+            lo[x] = h2bits(__floats2half2_rn(f.x - b.x, f.y - b.y));
+          }
+        }
+        *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (kq + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnParams p) {
   constexpr bool kLo = sizeof(T) == 4;
@@ -256,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
-    mbar_init(smem_addr(&bars.qfull), kQWarps);
+    mbar_init(smem_addr(&bars.qfull), kQWarps + kConvWarps);
     mbar_init(smem_addr(&bars.qempty), 1 + kSoftWarps);     // the last S, and every reader of s_scl
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&bars.sfull[i]), 1);
@@ -345,6 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             const uint32_t x = 2 * (kc0 + (kLo ? t - 2 : (t - 2) >> 1)) + 1, slot = x % kSlots;
             if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
             if (ok && t < 4 && oc[i] > 0) ok = warp_wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
+            // the next S's keys are looked for before P, so that S follows PV at
+            // once; f32 rows' keys come into the slot that this PV gives up
+            if (!kLo && ok && i == 0 && t < n_steps) {
+              const uint32_t xk = 2 * (kc0 + (t >> 1));
+              ok = warp_wait(bars.full[xk % kSlots], (xk / kSlots) & 1, p.status);
+            }
             if (ok) ok = warp_wait(bars.pfull[i], sp[i] & 1, p.status);
             ++sp[i];
             if (!ok) break;
@@ -363,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           }
           if (t < n_steps) {
             const uint32_t x = 2 * (kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
-            if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
+            if (kLo || t == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
             if (!ok) break;
             tc_fence_after();
             const uint64_t b = op_desc + slot * (kOpBytes >> 4), a0 = q_desc + (kLo ? 0 : i) * (kOpBytes >> 4);
@@ -426,90 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         wait(bars.rfull[x % kRawStages], (x / kRawStages) & 1, p.status);
     } else if (warp >= kQ0) {
       // -------------------------------------------------------- query rows
-      // eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
-      // kq + 12 of row kr: the eight lanes of a 16-byte store phase write 128
-      // contiguous bytes.  Batches of eight rows are loaded together, the
-      // first before the wait for the queries' place.
-      constexpr uint32_t kVec = kLo ? 8 : 4, kBatch = kLo ? 2 : 4, kGroups = MR / 8 / kQWarps;
-      const uint32_t qw = warp - kQ0, kr = lane & 7, kq = lane >> 3;
       uint32_t item = 0;
       while (ok && walk.next()) {
-        const Piece &pc = walk.p;
-        const uint32_t n_rows = pc.s.nq * p.group;
-        uint4 raw[kBatch][kVec];
-        auto load_q = [&](uint32_t j0) {
-#pragma unroll
-          for (uint32_t j = 0; j < kBatch; ++j) {
-            const uint32_t row = pc.rt * MR + 8 * (qw + kQWarps * (j0 + j)) + kr, tok = row / p.group, hd = row % p.group;
-            const T *qp = static_cast<const T *>(p.q) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.q_stride +
-                          (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head + 8 * kq;
-#pragma unroll
-            for (uint32_t k = 0; k < kVec; ++k)
-              raw[j][k] = row < n_rows ? __ldg(reinterpret_cast<const uint4 *>(qp + (kLo ? 32 * (k / 2) + 4 * (k & 1) : 32 * k)))
-                                       : make_uint4(0u, 0u, 0u, 0u);
-          }
-        };
-        load_q(0);
-        if (item > 0) ok = warp_wait(bars.qempty, (item - 1) & 1, p.status);
-        if (!ok) break;
-#pragma unroll 1
-        for (uint32_t j0 = 0; j0 < kGroups; j0 += kBatch) {
-          if (j0) load_q(j0);
-#pragma unroll
-          for (uint32_t j = 0; j < kBatch; ++j) {
-            const uint32_t g = qw + kQWarps * (j0 + j);
-            float amax = 0.f;
-#pragma unroll
-            for (uint32_t k = 0; k < kVec; ++k) {
-              const uint32_t u[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                if (kLo) {
-                  amax = fmaxf(amax, fabsf(__uint_as_float(u[x])));
-                } else {
-                  const float2 f = pair_of<T>(u[x]);
-                  amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-                }
-              }
-            }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-            int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-            e = e < -100 ? -100 : e > 110 ? 110 : e;
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-            if (kq == 0)
-              s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            uint8_t *dst = smem + kOffQ + kSbo * g + 16 * kr;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t hi[4], lo[4];
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                float2 f;
-                if (kLo) {
-                  const uint4 u = raw[j][kLo ? 2 * k + (x >> 1) : 0];
-                  f = x & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
-                            : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-                } else {
-                  const uint4 u = raw[j][k];
-                  f = pair_of<T>(x == 0 ? u.x : x == 1 ? u.y : x == 2 ? u.z : u.w);
-                }
-                f.x *= down, f.y *= down;
-                const __half2 h = __floats2half2_rn(f.x, f.y);
-                hi[x] = h2bits(h);
-                if (kLo) {
-                  const float2 b = __half22float2(h);
-                  lo[x] = h2bits(__floats2half2_rn(f.x - b.x, f.y - b.y));
-                }
-              }
-              *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (kq + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
+        ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
+        if (ok) load_queries<T>(p, walk.p, smem + kOffQ, s_scl, warp - kQ0);
+        if (ok && lane == 0) mbar_arrive(smem_addr(&bars.qfull));
         ++item;
       }
     } else if (warp >= kConv0) {
@@ -526,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&bars.full[x % kSlots]));
       };
-      uint32_t kc = 0;
+      uint32_t kc = 0, item = 0;
       while (ok && walk.next()) {
         const uint32_t n = walk.p.t1 - walk.p.t0;
         for (uint32_t t = 0; t < n; ++t, ++kc) {
@@ -555,6 +568,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
               }
             }
           hand_over(x);
+          // the piece's first keys are on their way while the queries' place
+          // is still taken; then this warp's share of the rows
+          if (t == 0) {
+            ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
+            if (!ok) break;
+            load_queries<T>(p, walk.p, smem + kOffQ, s_scl, kQWarps + cw);
+            if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
+            ++item;
+          }
           // values, transposed: row = dim 32 g + 8 s + r, keys 64 h + 16 cw + 8 u + 2 c and + 1
           ok = slot_free(x + 1);
           if (!ok) break;
@@ -727,10 +749,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         const bool none = M == -INFINITY && L == 0.f;
         float *part = p.part + (2ull * blockIdx.x + (pc.t0 == 0 ? 1 : 0)) * kPartFloats;
         // 32 dims at a time: f32 rows share the row's dims between the streams' warps
+        const uint32_t q0 = kLo ? 2 * i : 0, q1 = kLo ? 2 * i + 2 : 4;
+        uint32_t v[32];
+        tmem_ld32(o_col + (kLo ? 0 : 128 * i) + 32 * q0, v);
 #pragma unroll 1
-        for (uint32_t q = kLo ? 2 * i : 0; q < (kLo ? 2 * i + 2 : 4u); ++q) {
-          uint32_t v[32];
-          tmem_ld32(o_col + (kLo ? 0 : 128 * i) + 32 * q, v);
+        for (uint32_t q = q0; q < q1; ++q) {
           tmem_ld_wait32(v);
           float o[32];
 #pragma unroll
@@ -741,6 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = fmaf(__uint_as_float(v[x]), w1, o[x]);
           }
+          if (q + 1 < q1) tmem_ld32(o_col + (kLo ? 0 : 128 * i) + 32 * (q + 1), v);
           if (whole) {
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : o[x] * inv;
