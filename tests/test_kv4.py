@@ -19,7 +19,7 @@ def k_bits(t, dim):
 
 def v_bits(t, dim):
     g, s, r = dim // 32, dim % 32 // 8, dim % 8
-    at = 8 * (1024 + 512 * (t // 8) + 16 * (4 * r + t % 8 // 2) + 4 * g + 2 * (t % 2))
+    at = 8 * (1152 + 512 * (t // 8) + 16 * (4 * r + t % 8 // 2) + 4 * g + 2 * (t % 2))
     return [at + (([6, 2, 10, 14][s] + b) % 16) for b in range(4)]
 
 
@@ -31,7 +31,7 @@ def test_tile_layout_is_a_bijection_with_whole_bytes_per_token():
                 assert b not in seen
                 seen.add(b)
                 assert owner.setdefault(b // 8, t) == t
-    assert seen == set(range(8 * 2048))
+    assert seen == set(range(8 * 1024)) | set(range(8 * 1152, 8 * 2176))
     scale = {2 * (2 * (16 * (t // 8) + 4 * (t % 8 // 2) + g) + t % 2) for t in range(16) for g in range(4)}
     assert scale == set(range(0, 128, 2))
 

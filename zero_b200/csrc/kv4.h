@@ -14,13 +14,13 @@
 // q is chosen against the d that is stored.
 //
 // Storage is by tiles of 16 tokens of one kv head, 2304 contiguous bytes (one
-// bulk copy): K nibbles (1024), V nibbles (1024), K scales (128), V scales
-// (128), with n = q + 8 as the nibble.
+// bulk copy, or one for each half): K nibbles (1024), K scales (128), V nibbles
+// (1024), V scales (128), with n = q + 8 as the nibble.
 //   K: token t's row is bytes 64 t..; word g of column c (bytes 64 t + 16 c +
 //      4 g) holds dims 32 g + 8 c + 0..7, even dims in its low half and odd
 //      dims in its high half, bits 4 s of a half being dim pair 2 s.
 //   V: half p = t / 8, column c = (t % 8) / 2, odd = t % 2; the 16 bits at
-//      512 p + 16 (4 r + c) + 4 g + 2 odd hold dims 32 g + 8 s + r, s = 0..3:
+//      512 p + 16 (4 r + c) + 4 g + 2 odd of its half hold dims 32 g + 8 s + r, s = 0..3:
 //      s = 0 at bits 6..9, 1 at 2..5, 2 at 10..13, 3 at 14, 15, 0, 1 (after a
 //      swap of the two bytes, 2 is at 2..5 and 3 at 6..9).
 //   Scales of K and of V: half index 2 (16 p + 4 c + g) + odd.
@@ -41,7 +41,7 @@ namespace zgpu {
 constexpr uint32_t kKv4Head = 128;          // head_dim
 constexpr uint32_t kKv4Tile = 16;           // tokens per tile
 constexpr uint32_t kKv4TileBytes = 2304;
-constexpr uint32_t kKv4V = 1024, kKv4Ks = 2048, kKv4Vs = 2176;   // offsets in a tile
+constexpr uint32_t kKv4Ks = 1024, kKv4V = 1152, kKv4Vs = 2176;   // offsets in a tile
 constexpr uint32_t kKv4MaxSeqs = 1024;
 constexpr uint32_t kKv4NoSlot = 0xFFFFFFFFu;
 // The largest scale: 24 d has to be finite in binary16 (the dequantising fma

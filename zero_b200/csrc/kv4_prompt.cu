@@ -49,12 +49,14 @@ static_assert(32 * (kQ0 + kQWarps) == kThreads, "every warp has a role");
 constexpr uint32_t kKeys = 128;                       // keys of a tile
 constexpr uint32_t kOpBytes = 128 * kKv4Head * 2;     // one operand tile: 128 rows x 128 binary16
 constexpr uint32_t kSlots = 3;                        // operand tiles of keys and values, in turn
-constexpr uint32_t kRawBytes = kKeys / kKv4Tile * kKv4TileBytes, kRawStages = 2;
+constexpr uint32_t kHalfBytes = kKv4TileBytes / 2;    // K's or V's words and scales of 16 keys
+constexpr uint32_t kRawBytes = kKeys / kKv4Tile * kHalfBytes, kRawStages = 2;   // of each kind
 constexpr uint32_t kOffQ = 0, kOffOp = 2 * kOpBytes, kOffRaw = kOffOp + kSlots * kOpBytes;
-constexpr uint32_t kOffTab = kOffRaw + kRawStages * kRawBytes;
+constexpr uint32_t kOffTab = kOffRaw + 2 * kRawStages * kRawBytes;
 constexpr uint32_t kMaxRows = 256;
 constexpr uint32_t kPartFloats = kMaxRows * (kKv4Head + 2);
-constexpr uint32_t kMinTiles = 2;                     // key tiles a range is worth
+constexpr uint32_t kPieceCost = 2;                    // what a piece costs beside its key tiles, in key tiles
+constexpr uint32_t kMinTiles = 2;                     // units of work that a range is worth
 constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemCols = 512;
 // kind::f16: D f32, A and B binary16, both K-major, N = 128, M = 128
 constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -62,7 +64,7 @@ constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24
 constexpr uint32_t kLbo = 128, kSbo = 2048;
 
 struct Bars {
-  uint64_t qfull, qempty, rfull[kRawStages], rempty[kRawStages], full[kSlots], empty[kSlots];
+  uint64_t qfull, qempty, rfull[2][kRawStages], rempty[2][kRawStages], full[kSlots], empty[kSlots];
   uint64_t sfull[2], pfull[2], ofull[2], oempty[2], join, drain;
 };
 
@@ -126,12 +128,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t &bar, uint32_t parity, uint32
   return __all_sync(0xffffffffu, wait(bar, parity, status));
 }
 
-// Walks the pieces of a range; every warp walks for itself.
+// Walks the pieces of a range; every warp walks for itself.  A piece of n key
+// tiles is n + kPieceCost units of work, the tiles being the last n.
 struct Piece {
   uint32_t seq, head, rt;        // what
   uint32_t t0, t1, n;            // key tiles t0 .. t1 - 1 of n
   Kv4Seq s;
-  uint64_t at;                   // the piece's start in units of work
+  uint64_t at;                   // the piece's first tile in units of work
 };
 
 template <uint32_t MR>
@@ -141,7 +144,7 @@ struct Walk {
   uint32_t n_kv, group;
   uint64_t at, end;
   Piece p;
-  uint32_t n_rt;
+  uint32_t n_rt, off;            // units of the piece before `at`
   bool fresh;
 
   __device__ __forceinline__ static uint32_t row_tiles(uint32_t nq, uint32_t group) { return (nq * group + MR - 1) / MR; }
@@ -150,6 +153,10 @@ struct Walk {
     const uint32_t toks = min(nq, ((rt + 1) * MR - 1) / group + 1);    // tokens up to the tile's last row's
     const int64_t see = static_cast<int64_t>(len) - nq + toks;
     return see > 0 ? static_cast<uint32_t>((see + kKeys - 1) / kKeys) : 0u;
+  }
+  __device__ __forceinline__ static uint32_t units(uint32_t len, uint32_t nq, uint32_t group, uint32_t rt) {
+    const uint32_t n = tiles(len, nq, group, rt);
+    return n ? n + kPieceCost : 0u;
   }
   __device__ __forceinline__ void load() {
     p.s.len = lens[p.seq];
@@ -169,11 +176,11 @@ struct Walk {
     while (sums[lo + 1] <= at) ++lo;
     p.seq = lo;
     load();
-    const uint64_t per_head = (sums[lo + 1] - sums[lo]) / n_kv, off = at - sums[lo];
-    p.head = static_cast<uint32_t>(off / per_head);
-    uint64_t rem = off % per_head;
+    const uint64_t per_head = (sums[lo + 1] - sums[lo]) / n_kv, rem0 = at - sums[lo];
+    p.head = static_cast<uint32_t>(rem0 / per_head);
+    uint64_t rem = rem0 % per_head;
     for (uint32_t r0 = 0; r0 < n_rt; r0 += 32) {
-      const uint32_t mine = r0 + lane < n_rt ? tiles(p.s.len, p.s.nq, group, r0 + lane) : 0u;
+      const uint32_t mine = r0 + lane < n_rt ? units(p.s.len, p.s.nq, group, r0 + lane) : 0u;
       uint32_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -184,39 +191,43 @@ struct Walk {
       if (hit) {
         const uint32_t l = __ffs(hit) - 1;
         p.rt = r0 + l;
-        p.n = __shfl_sync(0xffffffffu, mine, l);
-        p.t0 = static_cast<uint32_t>(rem) - (__shfl_sync(0xffffffffu, inc, l) - p.n);
+        p.n = __shfl_sync(0xffffffffu, mine, l) - kPieceCost;
+        off = static_cast<uint32_t>(rem) - (__shfl_sync(0xffffffffu, inc, l) - p.n - kPieceCost);
         break;
       }
       rem -= __shfl_sync(0xffffffffu, inc, 31);
     }
     fresh = true;
   }
-  // The next piece of the range, or false.
+  // The next piece of the range with a key tile in it, or false.
   __device__ __noinline__ bool next() {
-    if (at >= end) return false;
-    if (!fresh) {
-      p.t0 = 0;
-      while (true) {
-        if (++p.rt == n_rt) {
-          p.rt = 0;
-          if (++p.head == n_kv) {
-            p.head = 0;
-            do ++p.seq;
-            while (sums[p.seq + 1] <= at);
-            load();
+    while (at < end) {
+      if (!fresh) {
+        off = 0;
+        while (true) {
+          if (++p.rt == n_rt) {
+            p.rt = 0;
+            if (++p.head == n_kv) {
+              p.head = 0;
+              do ++p.seq;
+              while (sums[p.seq + 1] <= at);
+              load();
+            }
           }
+          p.n = tiles(p.s.len, p.s.nq, group, p.rt);
+          if (p.n) break;
         }
-        p.n = tiles(p.s.len, p.s.nq, group, p.rt);
-        if (p.n) break;
       }
+      fresh = false;
+      p.at = at - off + kPieceCost;
+      const uint64_t left = end - at;
+      const uint32_t last = left < p.n + kPieceCost - off ? off + static_cast<uint32_t>(left) : p.n + kPieceCost;
+      p.t0 = off > kPieceCost ? off - kPieceCost : 0u;
+      p.t1 = last > kPieceCost ? last - kPieceCost : 0u;
+      at += last - off;
+      if (p.t1 > p.t0) return true;
     }
-    fresh = false;
-    p.at = at - p.t0;
-    const uint64_t left = end - at;
-    p.t1 = left < p.n - p.t0 ? p.t0 + static_cast<uint32_t>(left) : p.n;
-    at += p.t1 - p.t0;
-    return true;
+    return false;
   }
 };
 
@@ -230,7 +241,7 @@ template <class T>
 __device__ __noinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
                                           uint32_t share) {
   constexpr bool kLo = sizeof(T) == 4, kCopy = __is_same(T, __half);
-  constexpr uint32_t MR = kLo ? 128 : 256, kVec = kLo ? 8 : 4, kBatch = kLo ? 1 : 3, kShares = kConvWarps + kQWarps;
+  constexpr uint32_t MR = kLo ? 128 : 256, kVec = kLo ? 8 : 4, kBatch = kLo ? 2 : 3, kShares = kConvWarps + kQWarps;
   const uint32_t lane = threadIdx.x & 31, kr = lane & 7, kq = lane >> 3, n_rows = pc.s.nq * p.group;
   const uint32_t seq_q0 = pc.s.q0, head = pc.head, row0 = pc.rt * MR;
 #pragma unroll 1
@@ -279,13 +290,9 @@ __device__ __noinline__ void load_queries(const Kv4AttnParams &p, const Piece &p
         s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (kCopy) {
-          *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = raw[j][k];
-          continue;
-        }
-        uint32_t hi[4], lo[4];
+        uint32_t hi[4] = {raw[j][kCopy ? k : 0].x, raw[j][kCopy ? k : 0].y, raw[j][kCopy ? k : 0].z, raw[j][kCopy ? k : 0].w}, lo[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < (kCopy ? 0 : 4); ++x) {
           float2 f;
           if (kLo) {
             const uint4 u = raw[j][kLo ? 2 * k + (x >> 1) : 0];
@@ -351,8 +358,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       mbar_init(smem_addr(&bars.oempty[i]), kLo ? kSoftWarps : kSoftWarps / 2);
     }
     for (uint32_t i = 0; i < kRawStages; ++i) {
-      mbar_init(smem_addr(&bars.rfull[i]), 1);
-      mbar_init(smem_addr(&bars.rempty[i]), kConvWarps);
+      for (uint32_t v = 0; v < 2; ++v) {
+        mbar_init(smem_addr(&bars.rfull[v][i]), 1);
+        mbar_init(smem_addr(&bars.rempty[v][i]), kConvWarps);
+      }
     }
     for (uint32_t i = 0; i < kSlots; ++i) {
       mbar_init(smem_addr(&bars.full[i]), kConvWarps);
@@ -376,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
   for (uint32_t i = warp; i < p.n_seq; i += kThreads / 32) {
     const uint32_t nq = nqs[i], n_rt = Walk<MR>::row_tiles(nq, p.group);
     uint64_t w = 0;
-    for (uint32_t r = lane; r < n_rt; r += 32) w += Walk<MR>::tiles(lens[i], nq, p.group, r);
+    for (uint32_t r = lane; r < n_rt; r += 32) w += Walk<MR>::units(lens[i], nq, p.group, r);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     if (lane == 0) sums[i + 1] = w * p.n_kv;
@@ -411,6 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     walk.start(p.n_seq);
     // steps of a piece with key tiles 0 .. n - 1: stream t & 1, key tile kv_of(t)
     auto steps = [](uint32_t n) { return kLo ? n : 2 * n; };
+    // The place of key tile j and of its values in the ring's order.  f32 rows
+    // ask for K(t + 2) right behind PV(t): their keys come two tiles before
+    // their values (K0 K1 V0 K2 V1 ..), or they would wait for PV(t)'s slot;
+    // 16-bit rows' come in turn (K0 V0 K1 V1 ..).
+    auto key_tile = [](uint32_t j) { return kLo ? (j < 2 ? j : 2 * j - 1) : 2 * j; };
+    auto value_tile = [](uint32_t j) { return kLo ? 2 * j + 2 : 2 * j + 1; };
     bool ok = true;
 
     if (warp == kMmaWarp) {
@@ -420,7 +435,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
       const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
       const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
-      // operand tile x of the ring: key tile kc is x = 2 kc, its values 2 kc + 1
       while (ok && walk.next()) {
         const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
         ok = warp_wait(bars.qfull, item & 1, p.status);
@@ -428,13 +442,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
           const uint32_t i = t & 1, d = tmem + kTmemO + 128 * i, sc = tmem + kTmemS + 128 * i;
           if (t >= 2 && t - 2 < n_steps) {
-            const uint32_t x = 2 * (kc0 + (kLo ? t - 2 : (t - 2) >> 1)) + 1, slot = x % kSlots;
+            const uint32_t x = value_tile(kc0 + (kLo ? t - 2 : (t - 2) >> 1)), slot = x % kSlots;
             if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
             if (ok && t < 4 && oc[i] > 0) ok = warp_wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
-            // the next S's keys are looked for before P, so that S follows PV at
-            // once; f32 rows' keys come into the slot that this PV gives up
-            if (!kLo && ok && i == 0 && t < n_steps) {
-              const uint32_t xk = 2 * (kc0 + (t >> 1));
+            // the next S's keys are looked for before P, so that S follows PV at once
+            if (ok && (kLo || i == 0) && t < n_steps) {
+              const uint32_t xk = key_tile(kc0 + (kLo ? t : t >> 1));
               ok = warp_wait(bars.full[xk % kSlots], (xk / kSlots) & 1, p.status);
             }
             if (ok) ok = warp_wait(bars.pfull[i], sp[i] & 1, p.status);
@@ -454,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             __syncwarp();
           }
           if (t < n_steps) {
-            const uint32_t x = 2 * (kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
-            if (kLo || t == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
+            const uint32_t x = key_tile(kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
+            if (t == 0 || (kLo && t == 1)) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
             if (!ok) break;
             tc_fence_after();
             const uint64_t b = op_desc + slot * (kOpBytes >> 4), a0 = q_desc + (kLo ? 0 : i) * (kOpBytes >> 4);
@@ -485,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // ------------------------------------------ the key tiles' 4-bit words
       // lane h < 8: keys 16 h .. of the tile, table entries a tile ahead
       const uint32_t tpb_log2 = p.bt_log2 - 4;
-      uint32_t kc = 0;
+      uint32_t kc = 0, issued[2] = {0, 0};
       while (ok && walk.next()) {
         const Piece &pc = walk.p;
         const uint32_t *table = p.table + static_cast<size_t>(pc.seq) * p.table_width;
@@ -501,21 +514,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           const uint8_t *src = p.pool + (((static_cast<size_t>(there ? ent : 0u) * p.n_kv + pc.head) << tpb_log2) +
                                          (tile & ((1u << tpb_log2) - 1u))) * kKv4TileBytes;
           ent = entry(t + 1);
-          if (kc >= kRawStages) ok = warp_wait(bars.rempty[stage], (kc / kRawStages - 1) & 1, p.status);
-          if (!ok) break;
           if (lane < 8) s_bad[kc & 7][lane] = bad;
           if (bad) atomicOr(p.status, ZDEV_ERR_BOUNDS);
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(smem_addr(&bars.rfull[stage]), kRawBytes);
-          __syncwarp();
-          if (lane < 8)
-            bulk_copy_g2s(smem_addr(smem) + kOffRaw + stage * kRawBytes + lane * kKv4TileBytes, src, kKv4TileBytes,
-                          smem_addr(&bars.rfull[stage]));
+#pragma unroll 1
+          for (uint32_t v = 0; ok && v < 2; ++v) {
+            if (kc >= kRawStages) ok = warp_wait(bars.rempty[v][stage], (kc / kRawStages - 1) & 1, p.status);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(smem_addr(&bars.rfull[v][stage]), kRawBytes);
+            __syncwarp();
+            if (lane < 8)
+              bulk_copy_g2s(smem_addr(smem) + kOffRaw + (v * kRawStages + stage) * kRawBytes + lane * kHalfBytes,
+                            src + v * kHalfBytes, kHalfBytes, smem_addr(&bars.rfull[v][stage]));
+            issued[v] = kc + 1;
+          }
+          if (!ok) break;
         }
       }
       // never leave a copy in flight when the CTA may exit
-      for (uint32_t x = kc > kRawStages ? kc - kRawStages : 0; x < kc; ++x)
-        wait(bars.rfull[x % kRawStages], (x / kRawStages) & 1, p.status);
+      for (uint32_t v = 0; v < 2; ++v)
+        for (uint32_t x = issued[v] > kRawStages ? issued[v] - kRawStages : 0; x < issued[v]; ++x)
+          wait(bars.rfull[v][x % kRawStages], (x / kRawStages) & 1, p.status);
     } else if (warp >= kQ0) {
       // -------------------------------------------------------- query rows
       uint32_t item = 0;
@@ -539,70 +557,84 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&bars.full[x % kSlots]));
       };
+      // this warp's sixteen keys of each half of tile j: 16 (4 h + cw) ..
+      auto raw_ready = [&](uint32_t v, uint32_t j) { return warp_wait(bars.rfull[v][j % kRawStages], (j / kRawStages) & 1, p.status); };
+      auto raw_of = [&](uint32_t v, uint32_t j) {
+        return smem + kOffRaw + (v * kRawStages + j % kRawStages) * kRawBytes + cw * kHalfBytes;
+      };
+      auto raw_done = [&](uint32_t v, uint32_t j) {
+        if (lane == 0) mbar_arrive(smem_addr(&bars.rempty[v][j % kRawStages]));
+      };
+      auto keys = [&](uint32_t j) -> bool {
+        const uint32_t x = key_tile(j);
+        if (!raw_ready(0, j) || !slot_free(x)) return false;
+        // row = key 64 h + 16 cw + 8 u + kr, chunk 4 g + kq
+        uint8_t *kd = smem + kOffOp + (x % kSlots) * kOpBytes + kSbo * (2 * cw) + 16 * kr + kLbo * kq;
+#pragma unroll 1
+        for (int hu = 0; hu < 4; ++hu) {
+          const int h = hu >> 1, u = hu & 1;
+          const uint8_t *src = raw_of(0, j) + 4 * h * kHalfBytes;
+          const uint4 kw = *reinterpret_cast<const uint4 *>(src + 512 * u + 64 * kr + 16 * kq);
+          const uint4 ks = *reinterpret_cast<const uint4 *>(src + kKv4Ks + 64 * u + 16 * (kr >> 1));
+          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w}, s4[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const __half2 dd = bits2h(s4[g]);
+            const __half2 d = kr & 1 ? __high2half2(dd) : __low2half2(dd);
+            uint32_t v[4];
+            k_values(w[g], d, kg, v);
+            *reinterpret_cast<uint4 *>(kd + kSbo * (8 * h + u) + kLbo * 4 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        hand_over(x);
+        raw_done(0, j);
+        return true;
+      };
+      // transposed: row = dim 32 g + 8 s + r, keys 64 h + 16 cw + 8 u + 2 c and + 1
+      auto values = [&](uint32_t j) -> bool {
+        const uint32_t x = value_tile(j);
+        if (!raw_ready(1, j) || !slot_free(x)) return false;
+        uint8_t *vd = smem + kOffOp + (x % kSlots) * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
+#pragma unroll 1
+        for (int hu = 0; hu < 4; ++hu) {
+          const int h = hu >> 1, u = hu & 1;
+          const uint8_t *src = raw_of(1, j) + 4 * h * kHalfBytes;
+          const uint4 vw = *reinterpret_cast<const uint4 *>(src + 512 * u + 16 * lane);
+          const uint4 vs = *reinterpret_cast<const uint4 *>(src + (kKv4Vs - kKv4V) + 64 * u + 16 * c);
+          const uint32_t w[4] = {vw.x, vw.y, vw.z, vw.w}, s4[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const __half2 d = bits2h(s4[g]);
+            uint32_t v[4];
+            v_values(w[g], d, __hmul2(d, __float2half2_rn(-24.f)), mg, v);
+#pragma unroll
+            for (int s2 = 0; s2 < 4; ++s2)
+              *reinterpret_cast<uint32_t *>(vd + kLbo * (8 * h + u) + kSbo * (4 * g + s2)) = v[s2];
+          }
+        }
+        hand_over(x);
+        raw_done(1, j);
+        return true;
+      };
       uint32_t kc = 0, item = 0;
       while (ok && walk.next()) {
         const uint32_t n = walk.p.t1 - walk.p.t0;
-        for (uint32_t t = 0; t < n; ++t, ++kc) {
-          const uint32_t stage = kc % kRawStages, x = 2 * kc;
-          ok = warp_wait(bars.rfull[stage], (kc / kRawStages) & 1, p.status) && slot_free(x);
-          if (!ok) break;
-          // this warp's sixteen keys of each half of the tile: 16 (4 h + cw) ..
-          const uint8_t *raw = smem + kOffRaw + stage * kRawBytes + cw * kKv4TileBytes;
-          // keys: row = key 64 h + 16 cw + 8 u + kr, chunk 4 g + kq
-          uint8_t *kd = smem + kOffOp + (x % kSlots) * kOpBytes + kSbo * (2 * cw) + 16 * kr + kLbo * kq;
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-            for (int u = 0; u < 2; ++u) {
-              const uint8_t *src = raw + 4 * h * kKv4TileBytes;
-              const uint4 kw = *reinterpret_cast<const uint4 *>(src + 512 * u + 64 * kr + 16 * kq);
-              const uint4 ks = *reinterpret_cast<const uint4 *>(src + kKv4Ks + 64 * u + 16 * (kr >> 1));
-              const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w}, s4[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const __half2 dd = bits2h(s4[g]);
-                const __half2 d = kr & 1 ? __high2half2(dd) : __low2half2(dd);
-                uint32_t v[4];
-                k_values(w[g], d, kg, v);
-                *reinterpret_cast<uint4 *>(kd + kSbo * (8 * h + u) + kLbo * 4 * g) = make_uint4(v[0], v[1], v[2], v[3]);
-              }
-            }
-          hand_over(x);
+        for (uint32_t t = 0; ok && t < n; ++t, ++kc) {
+          ok = keys(kc);
+          if (ok && (!kLo || kc > 0) && !(!kLo && t == 0)) ok = values(kLo ? kc - 1 : kc);
           // the piece's first keys are on their way while the queries' place
           // is still taken; then this warp's share of the rows
-          if (t == 0) {
+          if (ok && t == 0) {
             ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
             if (!ok) break;
             load_queries<T>(p, walk.p, smem + kOffQ, s_scl, kQWarps + cw);
             if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
             ++item;
+            if (!kLo) ok = values(kc);
           }
-          // values, transposed: row = dim 32 g + 8 s + r, keys 64 h + 16 cw + 8 u + 2 c and + 1
-          ok = slot_free(x + 1);
-          if (!ok) break;
-          uint8_t *vd = smem + kOffOp + ((x + 1) % kSlots) * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-            for (int u = 0; u < 2; ++u) {
-              const uint8_t *src = raw + 4 * h * kKv4TileBytes + kKv4V;
-              const uint4 vw = *reinterpret_cast<const uint4 *>(src + 512 * u + 16 * lane);
-              const uint4 vs = *reinterpret_cast<const uint4 *>(src + (kKv4Vs - kKv4V) + 64 * u + 16 * c);
-              const uint32_t w[4] = {vw.x, vw.y, vw.z, vw.w}, s4[4] = {vs.x, vs.y, vs.z, vs.w};
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const __half2 d = bits2h(s4[g]);
-                uint32_t v[4];
-                v_values(w[g], d, __hmul2(d, __float2half2_rn(-24.f)), mg, v);
-#pragma unroll
-                for (int s2 = 0; s2 < 4; ++s2)
-                  *reinterpret_cast<uint32_t *>(vd + kLbo * (8 * h + u) + kSbo * (4 * g + s2)) = v[s2];
-              }
-            }
-          hand_over(x + 1);
-          if (lane == 0) mbar_arrive(smem_addr(&bars.rempty[stage]));
         }
       }
+      if (ok && kLo && kc > 0) values(kc - 1);
     } else {
       // ------------------------------------------------------------ softmax
       const uint32_t i = warp >> 2, row = 32 * (warp & 3) + lane;     // stream, row of the stream
