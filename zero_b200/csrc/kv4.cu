@@ -223,14 +223,21 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
 }
 
-// The integer nearest to x / d (ties to even), clamped to -8..7, plus 8.  The
-// quotient is rounded from an approximate reciprocal and then put right from
-// the remainder x - r d, which the fma gives exactly: it is a multiple of
-// both last places and at most about |d|, so it has at most 24 bits.
-__device__ __forceinline__ uint32_t nibble(float x, float d, float inv) {
+// The larger magnitude, NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+// n = q + 8 of one value where the quick rounding of x / d cannot be trusted:
+// r is within one of the quotient, and the remainder x - r d, which the fma
+// gives exactly (a multiple of both last places and at most about |d|, so at
+// most 24 bits), says on which side of a border x lies.
+__device__ __forceinline__ uint32_t nibble_exact(float x, float d, float inv) {
   float r = rintf(x * inv);
   const float e = fmaf(-r, d, x), h = 0.5f * fabsf(d);
-  if (fabsf(e) >= h && d != 0.f) {
+  if (fabsf(e) >= h) {
     const float r1 = r + ((e > 0.f) == (d > 0.f) ? 1.f : -1.f);
     if (fabsf(e) > h || (static_cast<int>(r) & 1)) r = r1;
   }
@@ -238,70 +245,63 @@ __device__ __forceinline__ uint32_t nibble(float x, float d, float inv) {
   return static_cast<uint32_t>(static_cast<int>(r) + 8);
 }
 
-// One row of 128 values, four per lane, eight lanes per group: the four
-// nibbles in bits 0..15 (element e at 4 e) and the group's scale.  A group
-// that cannot be held (a non-finite value, a magnitude above 8 * 2720) is
-// stored as zeros and recorded as a numerical error.
-__device__ __forceinline__ uint32_t quantise4(float4 v, uint32_t lane, __half *scale, uint32_t *status) {
+// One row of 128 values, four per lane, eight lanes per group: the lane's four
+// n and the group's scale.  A group that cannot be held (a non-finite value, a
+// magnitude above 8 * 2720) is stored as zeros and recorded as a numerical
+// error.  The work is bound by instruction issue, so the common case is kept
+// short: x / d is rounded by adding 1.5 * 2^23, and only a warp in which some
+// remainder reaches d / 2 (a tie, or a quotient rounded onto a border) takes
+// the exact form.
+__device__ __forceinline__ void quantise4(float4 v, uint32_t lane, uint32_t (&n)[4], __half *scale, uint32_t *status) {
   const float x[4] = {v.x, v.y, v.z, v.w};
-  uint32_t a[4], amax = 0;
+  float amax = max_abs_nan(max_abs_nan(x[0], x[1]), max_abs_nan(x[2], x[3]));
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    a[e] = __float_as_uint(x[e]) & 0x7FFFFFFFu;
-    amax = max(amax, a[e]);
-  }
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  float m = 0.f;
-  bool has = false;
-#pragma unroll
-  for (int e = 3; e >= 0; --e)
-    if (a[e] == amax) {
-      m = x[e];
-      has = true;
-    }
-  const uint32_t base = lane & 24u;
-  const uint32_t who = (__ballot_sync(0xffffffffu, has) >> base) & 0xFFu;
-  m = __shfl_sync(0xffffffffu, m, base + __ffs(who) - 1);
-  __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(m * -0.125f)));
-  float d = __half2float(dh);
-  if (amax >= 0x7F800000u || !(fabsf(d) <= kKv4MaxScale)) {
-    if (lane == base) atomicOr(status, ZDEV_ERR_NUMERICAL);
+  for (int off = 1; off < 8; off <<= 1) amax = max_abs_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  // the sign of the first value of that magnitude
+  const bool has[4] = {fabsf(x[0]) == amax, fabsf(x[1]) == amax, fabsf(x[2]) == amax, fabsf(x[3]) == amax};
+  const float mine = has[0] ? x[0] : has[1] ? x[1] : has[2] ? x[2] : x[3];
+  const uint32_t any = __ballot_sync(0xffffffffu, has[0] || has[1] || has[2] || has[3]);
+  const uint32_t below = __ballot_sync(0xffffffffu, mine < 0.f), group = 0xFFu << (lane & 24u);
+  const uint32_t first = any & group & (0u - (any & group));     // the group's lowest lane that has it
+  float d = (first & below ? 0.125f : -0.125f) * amax;
+  __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(d)));
+  d = __half2float(dh);
+  if (!(fabsf(d) <= kKv4MaxScale) || !(amax < INFINITY)) {
+    if ((lane & 7u) == 0) atomicOr(status, ZDEV_ERR_NUMERICAL);
     d = 0.f;
     dh = __float2half_rn(0.f);
   }
   *scale = dh;
-  uint32_t n = 0x8888u;
-  if (d != 0.f) {
-    const float inv = 1.0f / d;
-    n = 0;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+  float worst = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) n |= nibble(x[e], d, inv) << (4 * e);
+  for (int e = 0; e < 4; ++e) {
+    const float t = fmaf(x[e], inv, 12582912.f), r = t - 12582912.f;
+    worst = fmaxf(worst, fabsf(fmaf(-r, d, x[e])));
+    n[e] = __vimin_s32_relu(__float_as_int(t) - (0x4B400000 - 8), 15);   // 0..15: a tiny scale may be far from m / 8
   }
-  return n;
+  if (__any_sync(0xffffffffu, !(worst < 0.5f * fabsf(d)))) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n[e] = d != 0.f ? nibble_exact(x[e], d, inv) : 8u;
+  }
 }
 
-// The four nibbles of one element index held by the four lanes of this
-// lane's parity in its group (a 4 x 4 transpose; its own inverse).
+// A 4 x 4 transpose of nibbles over the four lanes of this lane's parity in
+// its group (its own inverse): lane s's nibble e becomes lane e's nibble s.
 __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t n, uint32_t lane) {
-  const uint32_t base = lane & 25u, s = (lane >> 1) & 3u;
-  uint32_t out = 0;
-#pragma unroll
-  for (uint32_t j = 0; j < 4; ++j) {
-    const uint32_t o = __shfl_sync(0xffffffffu, n, base + 2 * j);
-    out |= ((o >> (4 * s)) & 15u) << (4 * j);
-  }
-  return out;
+  const uint32_t q = __shfl_xor_sync(0xffffffffu, n, 4);
+  n = __byte_perm(n, q, lane & 4u ? 0x7715u : 0x7740u) & 0xFFFFu;
+  const uint32_t p = __shfl_xor_sync(0xffffffffu, n, 2);
+  return lane & 2u ? (n & 0xF0F0u) | ((p >> 4) & 0x0F0Fu) : (n & 0x0F0Fu) | ((p << 4) & 0xF0F0u);
 }
 
-__device__ __forceinline__ uint32_t k_word_part(uint32_t n, uint32_t lane) {
-  const uint32_t w = (n & 15u) | (((n >> 8) & 15u) << 4) | (((n >> 4) & 15u) << 16) | ((n >> 12) << 20);
-  return lane & 1u ? w << 8 : w;
+// Nibble pairs (bits 0..3 and 16..19) as (n - 8) d, exact in binary16.
+__device__ __forceinline__ float2 pair_values(uint32_t n, __half2 d) {
+  const uint32_t x = (n & 0x000F000Fu) | 0x64006400u;      // 1024 + n
+  return __half22float2(__hmul2(__hadd2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0xE408))), d));
 }
-__device__ __forceinline__ uint32_t k_word_nibbles(uint32_t w, uint32_t lane) {
-  if (lane & 1u) w >>= 8;
-  return (w & 15u) | ((w >> 4) & 15u) << 8 | ((w >> 16) & 15u) << 4 | ((w >> 20) & 15u) << 12;
-}
+
 // Byte offsets in a tile: lane's K word (shared by two lanes) and 16 V bits of
 // token t, and the scale of its group g.
 __device__ __forceinline__ uint32_t v_off(uint32_t t, uint32_t lane) {
@@ -320,45 +320,58 @@ constexpr uint32_t kRowWarps = 8;
 // A warp per (token, kv head): rows in with 512-byte loads, 144 bytes out.
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t n = static_cast<uint64_t>(p.n_tokens) * p.n_kv;
-  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); i < n;
-       i += static_cast<uint64_t>(gridDim.x) * kRowWarps) {
-    const uint32_t token = static_cast<uint32_t>(i / p.n_kv), head = static_cast<uint32_t>(i % p.n_kv);
-    const uint32_t slot = p.slots[token];
+  // the number of warps is a multiple of n_kv: a warp keeps its head
+  const uint32_t lane = threadIdx.x & 31, w0 = blockIdx.x * kRowWarps + (threadIdx.x >> 5), head = w0 % p.n_kv;
+  const uint32_t step = gridDim.x * kRowWarps / p.n_kv;
+  uint32_t token = w0 / p.n_kv;
+  if (token >= p.n_tokens) return;
+  const T *kp = static_cast<const T *>(p.k) + head * kKv4Head + 4 * lane;
+  const T *vp = static_cast<const T *>(p.v) + head * kKv4Head + 4 * lane;
+  uint32_t next_slot = p.slots[token];
+  float4 next_k = load4(kp + token * p.k_stride), next_v = load4(vp + token * p.v_stride);
+  while (true) {
+    const uint32_t slot = next_slot;
+    const float4 kx = next_k, vx = next_v;
+    // the next token's rows are on their way while this one's are worked on
+    const bool more = p.n_tokens - token > step;
+    token += step;
+    if (more) {
+      next_slot = p.slots[token];
+      next_k = load4(kp + token * p.k_stride);
+      next_v = load4(vp + token * p.v_stride);
+    }
     if (slot >= p.n_slots) {
       if (slot != kKv4NoSlot && lane == 0) atomicOr(p.status, ZDEV_ERR_BOUNDS);
+      if (!more) return;
       continue;
     }
-    const float4 kx = load4(static_cast<const T *>(p.k) + token * p.k_stride + head * kKv4Head + 4 * lane);
-    const float4 vx = load4(static_cast<const T *>(p.v) + token * p.v_stride + head * kKv4Head + 4 * lane);
     uint8_t *tile = p.pool + kv4_tile_off(slot, head, p.n_kv, p.bt_log2);
     const uint32_t t = slot % kKv4Tile;
     __half ks, vs;
-    uint32_t w = k_word_part(quantise4(kx, lane, &ks, p.status), lane);
+    uint32_t kn[4], vn[4];
+    quantise4(kx, lane, kn, &ks, p.status);
+    quantise4(vx, lane, vn, &vs, p.status);
+    // two lanes make a K word: dims 0, 2 | 1, 3 of the one, 4, 6 | 5, 7 of the other
+    uint32_t w = kn[0] | kn[2] << 4 | kn[1] << 16 | kn[3] << 20;
+    if (lane & 1u) w <<= 8;
     w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    const uint32_t vn = transpose_nibbles(quantise4(vx, lane, &vs, p.status), lane);
+    const uint32_t vt = transpose_nibbles(vn[0] | vn[1] << 4 | vn[2] << 8 | vn[3] << 12, lane);
     if (!(lane & 1u)) *reinterpret_cast<uint32_t *>(tile + k_off(t, lane)) = w;
-    *reinterpret_cast<uint16_t *>(tile + v_off(t, lane)) = static_cast<uint16_t>(kv4_v_bits(vn));
+    *reinterpret_cast<uint16_t *>(tile + v_off(t, lane)) = static_cast<uint16_t>(kv4_v_bits(vt));
     if ((lane & 7u) == 0) {
       *reinterpret_cast<__half *>(tile + kKv4Ks + scale_off(t, lane / 8)) = ks;
       *reinterpret_cast<__half *>(tile + kKv4Vs + scale_off(t, lane / 8)) = vs;
     }
+    if (!more) return;
   }
-}
-
-__device__ __forceinline__ float4 dequant4(uint32_t n, float d) {
-  return make_float4((static_cast<int>(n & 15u) - 8) * d, (static_cast<int>((n >> 4) & 15u) - 8) * d,
-                     (static_cast<int>((n >> 8) & 15u) - 8) * d, (static_cast<int>((n >> 12) & 15u) - 8) * d);
 }
 
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4RowsParams p) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t n = static_cast<uint64_t>(p.n_tokens) * p.n_kv;
-  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); i < n;
-       i += static_cast<uint64_t>(gridDim.x) * kRowWarps) {
-    const uint32_t token = static_cast<uint32_t>(i / p.n_kv), head = static_cast<uint32_t>(i % p.n_kv);
+  // the number of warps is a multiple of n_kv: a warp keeps its head
+  const uint32_t lane = threadIdx.x & 31, w0 = blockIdx.x * kRowWarps + (threadIdx.x >> 5), head = w0 % p.n_kv;
+  const uint32_t step = gridDim.x * kRowWarps / p.n_kv;
+  for (uint32_t token = w0 / p.n_kv; token < p.n_tokens; token += step) {
     const uint32_t slot = p.slots[token];
     float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
     if (slot < p.n_slots) {
@@ -366,13 +379,17 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4Row
       const uint32_t t = slot % kKv4Tile;
       if (p.k_out) {
         const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + k_off(t, lane));
-        const __half d = *reinterpret_cast<const __half *>(tile + kKv4Ks + scale_off(t, lane / 8));
-        kx = dequant4(k_word_nibbles(w, lane), __half2float(d));
+        const __half2 d = __half2half2(*reinterpret_cast<const __half *>(tile + kKv4Ks + scale_off(t, lane / 8)));
+        const uint32_t mine = lane & 1u ? w >> 8 : w;
+        const float2 a = pair_values(mine, d), b = pair_values(mine >> 4, d);
+        kx = make_float4(a.x, a.y, b.x, b.y);
       }
       if (p.v_out) {
         const uint32_t u = *reinterpret_cast<const uint16_t *>(tile + v_off(t, lane));
-        const __half d = *reinterpret_cast<const __half *>(tile + kKv4Vs + scale_off(t, lane / 8));
-        vx = dequant4(transpose_nibbles(kv4_v_nibbles(u), lane), __half2float(d));
+        const __half2 d = __half2half2(*reinterpret_cast<const __half *>(tile + kKv4Vs + scale_off(t, lane / 8)));
+        const uint32_t n = transpose_nibbles(kv4_v_nibbles(u), lane);
+        const float2 a = pair_values(n | n << 12, d), b = pair_values(n >> 8 | (n >> 8) << 12, d);
+        vx = make_float4(a.x, a.y, b.x, b.y);
       }
     } else if (slot != kKv4NoSlot && lane == 0) {
       atomicOr(p.status, ZDEV_ERR_BOUNDS);
@@ -382,11 +399,15 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4Row
   }
 }
 
+// CTAs: eight per SM at most, and a number whose warps are a multiple of n_kv.
 uint32_t row_grid(const Kv4RowsParams &p, int sm_count) {
+  uint32_t unit = p.n_kv;
+  for (uint32_t k = 0; k < 3 && unit % 2 == 0; ++k) unit /= 2;      // n_kv / gcd(n_kv, 8)
   const uint64_t want = (static_cast<uint64_t>(p.n_tokens) * p.n_kv + kRowWarps - 1) / kRowWarps;
-  const uint64_t most = static_cast<uint64_t>(sm_count) * 8;
-  return static_cast<uint32_t>(want < most ? want : most);
+  const uint64_t most = static_cast<uint64_t>(sm_count) * 8, n = want < most ? want : most;
+  return static_cast<uint32_t>((n + unit - 1) / unit * unit);
 }
+static_assert(kRowWarps == 8, "row_grid");
 
 }  // namespace
 
