@@ -36,8 +36,9 @@
 //   barrier joins the warps until a piece of work ends.
 //
 //   Split.  All pieces of work (sequence, kv head, eight rows) are laid end to
-//   end in units of 32 keys and cut into equal ranges, one per CTA, so a
-//   ragged batch or one long sequence keeps every SM equally busy.  A piece
+//   end in units of 32 keys, each behind kPieceCost units for what a piece
+//   costs by itself (queries, merging), and cut into equal ranges, one per
+//   CTA, so a ragged batch or one long sequence keeps every SM equally busy.  A piece
 //   cut by a range boundary leaves unnormalised partials (max, sum, o) in the
 //   workspace; the CTA that arrives last merges them in range order, so the
 //   result does not depend on which one that is.
@@ -58,6 +59,7 @@ constexpr uint32_t kMergeRow = kKv4Head + 4;     // floats between a warp's rows
 constexpr uint32_t kMergeFloats = kRows * (kMergeRow + 2);
 constexpr float kPShift = 15.f;                  // P is held times 2^15
 constexpr uint32_t kMinUnits = kWarps / 2;       // a range is worth a unit for every second warp
+constexpr uint32_t kPieceCost = 16;              // what a piece costs beside its units, in units
 
 // Dynamic shared memory: the warps' rings, the warps' partials, the sums of
 // work over the sequences.
@@ -88,6 +90,21 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Units of a piece over len keys, its own cost included.
+__device__ __forceinline__ uint32_t units_of(uint32_t len) { return len ? (len + kUnit - 1) / kUnit + kPieceCost : 0u; }
+
+// a / b; the 64-bit division is long, and hardly ever needed.
+__device__ __noinline__ uint64_t long_div(uint64_t a, uint64_t b) { return a / b; }
+__device__ __forceinline__ uint64_t div64(uint64_t a, uint64_t b) {
+  return (a | b) >> 32 ? long_div(a, b) : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
+
+__device__ __forceinline__ uint32_t count_arrival(uint32_t *counter) {
+  uint32_t n;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
+  return n;
 }
 
 template <class T>
@@ -122,7 +139,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
         const Kv4Seq s = kv4_seq(p, i, &bad);
         blind |= s.len < s.nq;
         if (!p.few_only || s.nq * p.group <= kKv4FewRows)
-          w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * ((s.len + kUnit - 1) / kUnit);
+          w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * units_of(s.len);
       }
       uint64_t inc = w;
 #pragma unroll
@@ -162,8 +179,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     pdl_wait();
     return;
   }
-  uint64_t at = W * blockIdx.x / G;
-  const uint64_t end = W * (blockIdx.x + 1) / G;
+  uint64_t at = div64(W * blockIdx.x, G);
+  const uint64_t end = div64(W * (blockIdx.x + 1), G);
   uint32_t seq = 0;
   {
     uint32_t lo = 0, hi = p.n_seq;   // sums[lo] <= at < sums[hi]
@@ -182,13 +199,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     while (sums[seq + 1] <= at) ++seq;
     bool bad = false;
     const Kv4Seq s = kv4_seq(p, seq, &bad);
-    const uint32_t n_units = (s.len + kUnit - 1) / kUnit;
+    const uint32_t n_units = (s.len + kUnit - 1) / kUnit, all_units = n_units + kPieceCost;
     const uint32_t pieces = (s.nq * p.group + kRows - 1) / kRows;
-    const uint64_t piece = (at - sums[seq]) / n_units;
-    const uint64_t piece_at = sums[seq] + piece * n_units;   // the piece in units of work
-    const uint32_t head = static_cast<uint32_t>(piece / pieces), rt = static_cast<uint32_t>(piece % pieces);
-    const uint32_t t0 = static_cast<uint32_t>(at - piece_at);
-    const uint32_t t1 = static_cast<uint32_t>(end - piece_at < n_units ? end - piece_at : n_units);
+    const uint64_t piece = div64(at - sums[seq], all_units);
+    const uint64_t piece_at = sums[seq] + piece * all_units + kPieceCost;   // its first unit of keys
+    const uint32_t head = static_cast<uint32_t>(div64(piece, pieces)), rt = static_cast<uint32_t>(piece - static_cast<uint64_t>(head) * pieces);
+    const uint64_t piece_end = piece_at + n_units, stop = end < piece_end ? end : piece_end;
+    if (stop <= piece_at) break;        // the range ends in what the piece costs
+    const uint32_t t0 = at > piece_at ? static_cast<uint32_t>(at - piece_at) : 0u;
+    const uint32_t t1 = static_cast<uint32_t>(stop - piece_at);
+    // the queries' loads go first: warp w takes row w of the piece, four dims
+    // per lane (a row behind the last is the first one again, for no use)
+    const uint32_t n_rows = s.nq * p.group, qrow = rt * kRows + warp;
+    const uint32_t qtok = qrow < n_rows ? qrow / p.group : 0, qhd = qrow < n_rows ? qrow - qtok * p.group : 0;
+    const float4 qx = q4(static_cast<const T *>(p.q) + (s.q0 + qtok) * p.q_stride +
+                         (static_cast<size_t>(head) * p.group + qhd) * kKv4Head + 4 * lane);
     const uint32_t *table = p.table + static_cast<size_t>(seq) * p.table_width;
     const uint32_t tpb_log2 = p.bt_log2 - 4;
     // this warp's units: t0 + warp + 8 k, k < nk
@@ -238,14 +263,11 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     if (!dead)
       while (issued < ahead) issue();
 
-    // the queries: warp w takes row w of the piece, four dims per lane, scaled
-    // by a power of two and split in hi and lo; fragment kk of lane (r, c) is
-    // the 16 bytes at 512 kk + 16 lane: dims 32 (kk / 2) + 8 c + 4 (kk % 2) + 0..3
-    const uint32_t n_rows = s.nq * p.group;
+    // the queries, scaled by a power of two and split in hi and lo; fragment kk
+    // of lane (r, c) is the 16 bytes at 512 kk + 16 lane: dims 32 (kk / 2) + 8 c +
+    // 4 (kk % 2) + 0..3
     {
-      const uint32_t row = rt * kRows + warp, tok = row < n_rows ? row / p.group : 0, hd = row < n_rows ? row % p.group : 0;
-      const float4 x = q4(static_cast<const T *>(p.q) + (s.q0 + tok) * p.q_stride +
-                          (static_cast<size_t>(head) * p.group + hd) * kKv4Head + 4 * lane);
+      const float4 x = qx;
       float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
@@ -267,8 +289,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       if ((lane & 7u) == 0) s_bias[warp][lane >> 3] = qsum * (-8.f * 0x1p-24f);
       if (lane == 0) {
         // keys that the row sees: 0 .. limit - 1 (none when its position is negative)
-        const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + tok + 1;
-        // a row behind the last is the first one again, for no use
+        const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + qtok + 1;
         s_limit[warp] = pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
         s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + 24 - 8 + e) << 23);
       }
@@ -411,45 +432,41 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     __syncthreads();
     // thread: row mr, dims 4 mc ..
     const uint32_t mr = tid >> 5, mc = tid & 31;
+    // weights of states by their maxima: a state that saw no key has nothing
+    // to add, and a broken one (a NaN sum) breaks the whole
+    auto weight = [](float m, float top) { return m == top ? 1.f : ex2(m - top); };
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto fold = [&](float m, float l, float4 o) {
-      if (m == -INFINITY && l == 0.f) return;      // saw no key
-      const float nm = fmaxf(M, m), a = ex2(M - nm), b = ex2(m - nm);
-      L = L * a + l * b;
-      O.x = O.x * a + o.x * b;
-      O.y = O.y * a + o.y * b;
-      O.z = O.z * a + o.z * b;
-      O.w = O.w * a + o.w * b;
-      M = nm;
-    };
+    {
+      float2 ml[kWarps];
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      const float *src = merge + w * kMergeFloats;
-      fold(src[kRows * kMergeRow + 2 * mr], src[kRows * kMergeRow + 2 * mr + 1],
-           *reinterpret_cast<const float4 *>(src + mr * kMergeRow + 4 * mc));
+      for (uint32_t w = 0; w < kWarps; ++w) {
+        ml[w] = *reinterpret_cast<const float2 *>(merge + w * kMergeFloats + kRows * kMergeRow + 2 * mr);
+        M = fmaxf(M, ml[w].x);
+      }
+#pragma unroll
+      for (uint32_t w = 0; w < kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4 *>(merge + w * kMergeFloats + mr * kMergeRow + 4 * mc);
+        const float a = weight(ml[w].x, M);
+        L += ml[w].y * a;
+        O.x += x.x * a, O.y += x.y * a, O.z += x.z * a, O.w += x.w * a;
+      }
     }
     bool whole = t0 == 0 && t1 == n_units;
     if (!whole) {
       float *dst = p.part + (2ull * blockIdx.x + (t0 == 0 ? 1 : 0)) * kPartFloats;
       *reinterpret_cast<float4 *>(dst + mr * kKv4Head + 4 * mc) = O;
-      if (mc == 0) {
-        dst[kRows * kKv4Head + 2 * mr] = M;
-        dst[kRows * kKv4Head + 2 * mr + 1] = L;
-      }
-      __threadfence();
-      __syncthreads();
+      if (mc == 0) *reinterpret_cast<float2 *>(dst + kRows * kKv4Head + 2 * mr) = make_float2(M, L);
       // the ranges that share the piece
-      const uint32_t c0 = static_cast<uint32_t>(((piece_at + 1) * G - 1) / W);
-      const uint32_t c1 = static_cast<uint32_t>(((piece_at + n_units) * G - 1) / W);
+      const uint32_t c0 = static_cast<uint32_t>(div64((piece_at + 1) * G - 1, W));
+      const uint32_t c1 = static_cast<uint32_t>(div64(piece_end * G - 1, W));
+      __syncthreads();
       if (tid == 0) {
-        const uint32_t n = atomicAdd(&p.counters[c0], 1u);
-        s_last = n == c1 - c0;
+        s_last = count_arrival(&p.counters[c0]) == c1 - c0;
         if (s_last) p.counters[c0] = 0;
       }
       __syncthreads();
       if (s_last) {
-        __threadfence();
         // the row's largest maximum and the ranges' weights, a lane each, then
         // the sums: the loads of a batch do not wait for one another
         M = -INFINITY;
@@ -457,18 +474,14 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
         O = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t k0 = c0; k0 <= c1; k0 += 32) {
           const uint32_t k = k0 + mc;
-          float pm = -INFINITY, pl = 0.f;
-          if (k <= c1) {
-            const float *src = p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats + kRows * kKv4Head + 2 * mr;
-            pm = __ldcg(src);
-            pl = __ldcg(src + 1);
-          }
-          float nm = fmaxf(M, pm);
+          float2 st = make_float2(-INFINITY, 0.f);
+          if (k <= c1)
+            st = __ldcg(reinterpret_cast<const float2 *>(p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats +
+                                                         kRows * kKv4Head + 2 * mr));
+          float nm = fmaxf(M, st.x);
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, off));
-          const float keep = nm == -INFINITY ? 1.f : ex2(M - nm);
-          // a range that saw no key has nothing to add; a broken one (a NaN sum) has
-          const float w = pm == -INFINITY && pl == 0.f ? 0.f : ex2(pm - nm);
+          const float keep = weight(M, nm), w = weight(st.x, nm);
           L *= keep;
           O.x *= keep, O.y *= keep, O.z *= keep, O.w *= keep;
           const uint32_t n = min(32u, c1 - k0 + 1);
@@ -478,7 +491,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
             const float4 x = __ldcg(reinterpret_cast<const float4 *>(
                 p.part + (2ull * kj + (kj == c0 ? 1 : 0)) * kPartFloats + mr * kKv4Head + 4 * mc));
             const float wj = __shfl_sync(0xffffffffu, w, j);
-            L += __shfl_sync(0xffffffffu, pl, j) * wj;
+            L += __shfl_sync(0xffffffffu, st.y, j) * wj;
             O.x += x.x * wj, O.y += x.y * wj, O.z += x.z * wj, O.w += x.w * wj;
           }
           M = nm;
@@ -502,7 +515,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       }
     }
     __syncthreads();       // the merge area and s_last are free again
-    at = piece_at + t1;
+    at = stop;
   }
   pdl_wait();              // the launch ends no earlier than the one before it
 }
