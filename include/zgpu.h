@@ -302,16 +302,18 @@ typedef struct zgpu_kv4_work zgpu_kv4_work;
 zgpu_status zgpu_kv4_create(zgpu_ctx *ctx, uint32_t n_blocks, uint32_t block_tokens, uint32_t n_layers,
                             uint32_t n_kv_heads, uint32_t head_dim, zgpu_kv4 **out);
 void zgpu_kv4_destroy(zgpu_kv4 *kv);
-/* Scratch of the attention: one serves one call at a time.  Calls that may
- * overlap on the GPU (two streams, two graphs replayed side by side) need one
- * each. */
+/* Scratch of the attention (about 44 MB): one serves one call at a time.
+ * Calls that may overlap on the GPU (two streams, two graphs replayed side by
+ * side) need one each, and after ZGPU_ERR_DEVICE_TIMEOUT it has to be made
+ * again. */
 zgpu_status zgpu_kv4_work_create(zgpu_ctx *ctx, zgpu_kv4_work **out);
 void zgpu_kv4_work_destroy(zgpu_kv4_work *work);
-/* Waits for the context's stream, then reports and clears the first of the
- * errors that device calls recorded: ZGPU_ERR_KV_TOKEN_OUT_OF_RANGE (a slot,
- * block or length outside the cache), ZGPU_ERR_KV_TOKEN_COUNT_EXCEEDS_MAX (a
- * refused plan or release), ZGPU_ERR_NUMERICAL_INSTABILITY.  A caller that
- * used other streams waits for them first. */
+/* Waits for the context's stream, then clears the errors that device calls
+ * recorded and reports the first kind of them in this order:
+ * ZGPU_ERR_DEVICE_TIMEOUT, ZGPU_ERR_KV_TOKEN_OUT_OF_RANGE (a slot, block or
+ * length outside the cache), ZGPU_ERR_KV_TOKEN_COUNT_EXCEEDS_MAX (a refused
+ * plan or release), ZGPU_ERR_NUMERICAL_INSTABILITY.  A caller that used other
+ * streams waits for them first. */
 zgpu_status zgpu_kv4_check(zgpu_kv4 *kv);
 /* Plans one step of n_seq (1..1024) rows: row i holds d_old_lens[i] tokens and
  * gets d_new_lens[i] (0 allowed) more.  Blocks come from the end of
@@ -339,8 +341,9 @@ zgpu_status zgpu_kv4_release_device(zgpu_kv4 *kv, uint32_t n_seq, uint32_t table
                                     uint32_t *d_lens, uint32_t *d_table, uint32_t *d_free_list, uint32_t *d_state,
                                     void *stream);
 /* Quantises k and v rows [n_tokens][n_kv_heads * 128] into the slots of
- * d_slots [n_tokens]; a token with ZGPU_KV4_NONE is skipped.  No slot may be
- * named twice in one call. */
+ * d_slots [n_tokens]; a token with ZGPU_KV4_NONE is skipped (its rows are still
+ * there to be read).  No slot may be named twice in one call: it would be left
+ * with a mixture of the rows. */
 zgpu_status zgpu_kv4_append_device(zgpu_kv4 *kv, uint32_t layer, uint32_t n_tokens, const void *d_k, uint64_t k_stride,
                                    const void *d_v, uint64_t v_stride, uint32_t dtype, const uint32_t *d_slots,
                                    void *stream);

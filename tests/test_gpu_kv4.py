@@ -609,3 +609,101 @@ def test_attention_many_short_pieces_per_cta(ctx, dtype, n_seq, n):
     check_attn(c, o, q, dtype, rows=range(0, n_seq, max(1, n_seq // 6)))
     c["kv"].check()
     c["kv"].close()
+
+
+@pytest.mark.parametrize("nq", [1, 9])
+def test_attention_of_the_most_sequences(ctx, nq):
+    """1024 sequences, the largest table of sums; every 64th is checked."""
+    lens = [nq + (i * 37) % 90 for i in range(1024)]
+    c = make(ctx, 21, lens, [nq] * 1024, 4, 2, 16)
+    o, q = run_attn(c, "f32")
+    check_attn(c, o, q, "f32", rows=range(0, 1024, 64))
+    c["kv"].check()
+    c["kv"].close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_at_the_end_of_a_pool_of_many_gigabytes(ctx, dtype):
+    """Blocks whose bytes lie far beyond 2^32, single tokens and a chunk."""
+    n_kv, block, n_blocks = 8, 16, 300_000                  # 5.5 GB
+    kv = cache(ctx, n_blocks, block, 1, n_kv)
+    lens, nq, n_q = [70, 130], [1, 65], 16
+    rng = np.random.default_rng(4)
+    table = np.full((2, 10), NONE, np.uint32)
+    ids = n_blocks - 1 - rng.permutation(40)[:14]
+    table[0, :5], table[1, :9] = ids[:5], ids[5:14]
+    c = dict(kv=kv, table=table, lens=np.asarray(lens, np.uint32), starts=np.array([0, 1, 66], np.uint32), layer=0,
+             n_q=n_q, n_kv=n_kv, width=10, ks=[], vs=[], q=rng.standard_normal((66, n_q, HD)).astype(np.float32))
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        slots = (table[i][pos // block].astype(np.int64) * block + pos % block).astype(np.uint32)
+        k, v = (rng.standard_normal((n, n_kv, HD)).astype(np.float32) for _ in range(2))
+        store(kv, 0, slots, k, v)
+        c["ks"].append(R.values(k))
+        c["vs"].append(R.values(v))
+        gk, gv = fetch(kv, 0, slots, "f32", n_kv)
+        assert np.array_equal(gk, c["ks"][i]) and np.array_equal(gv, c["vs"][i])
+    o, q = run_attn(c, dtype)
+    check_attn(c, o, q, dtype)
+    kv.check()
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_sequences_that_share_blocks_and_rows_in_odd_order(ctx, dtype):
+    """Two sequences on one prefix's blocks, and a gap in the query rows."""
+    c = make(ctx, 31, [96, 200], [40, 1], 6, 2, 32)
+    c["table"][1, :3] = c["table"][0, :3]                  # 96 keys of the other sequence
+    c["ks"][1] = np.concatenate([c["ks"][0], c["ks"][1][96:]])
+    c["vs"][1] = np.concatenate([c["vs"][0], c["vs"][1][96:]])
+    o, q = run_attn(c, dtype)
+    check_attn(c, o, q, dtype)
+    c["kv"].check()
+    c["kv"].close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_attention_non_finite_16_bit_queries(ctx, dtype, value):
+    c = make(ctx, 9, [200, 90], [150, 1], 4, 2, 16)
+    c["q"][70, 1, 77] = value
+    o, q = run_attn(c, dtype)
+    with pytest.raises(zb.ZgpuError) as e:
+        c["kv"].check()
+    assert e.value.status == 20
+    assert np.isnan(o[70, 1]).all()
+    c["q"][70, 1] = 0
+    o0, _ = run_attn(c, dtype)
+    o[70, 1] = o0[70, 1] = 0
+    assert np.array_equal(o, o0)
+    c["kv"].close()
+
+
+def test_a_graph_of_each_of_two_chunks_replayed_side_by_side(ctx):
+    """Two captured calls with a workspace each, on two streams at once."""
+    c = make(ctx, 17, [700, 300], [200, 1], 8, 2, 16)
+    alone, _ = run_attn(c, "f16")
+    td = torch.float16
+    st, ln, tb, q = dev(c["starts"]), dev(c["lens"]), dev(c["table"]), dev(c["q"]).to(td)
+    outs, graphs, works = [torch.zeros_like(q) for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for o in outs:
+        works.append(c["kv"].new_work())
+        g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g, stream=s):
+            c["kv"].attention_device(0, 2, 201, 200, 8, q.data_ptr(), o.data_ptr(), st.data_ptr(), ln.data_ptr(),
+                                     tb.data_ptr(), c["width"], dtype=zb.F16, stream=s.cuda_stream, work=works[-1])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert np.array_equal(o.double().cpu().numpy(), alone)
+    del graphs
+    c["kv"].check()
+    for w in works:
+        w.close()
+    c["kv"].close()

@@ -294,7 +294,8 @@ class KvCache4:
             self.work.close()
 
     def __del__(self):
-        self.close()
+        if LIB is not None:      # the module may be gone first when the interpreter ends
+            self.close()
 
     def new_work(self) -> "KvCache4Work":
         return KvCache4Work(self.ctx)
@@ -355,7 +356,8 @@ class KvCache4Work:
             self.h = None
 
     def __del__(self):
-        self.close()
+        if LIB is not None:
+            self.close()
 
 
 class Qwen3Model:

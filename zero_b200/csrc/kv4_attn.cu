@@ -61,13 +61,13 @@ constexpr float kPShift = 15.f;                  // P is held times 2^15
 constexpr uint32_t kMinUnits = kWarps / 2;       // a range is worth a unit for every second warp
 constexpr uint32_t kPieceCost = 16;              // what a piece costs beside its units, in units
 
-// Dynamic shared memory: the warps' rings, the warps' partials, the sums of
-// work over the sequences.
+// Dynamic shared memory: the warps' rings (and, when a piece is done, the
+// warps' states in their places: two CTAs then fit an SM whatever the number of
+// sequences), the queries, the sums of work over the sequences.
 constexpr uint32_t kRingBytes = kWarps * kStages * kUnitBytes;
-constexpr uint32_t kMergeBytes = kWarps * kMergeFloats * 4;
+static_assert(kMergeFloats * 4 <= kStages * kUnitBytes, "a warp's state fits its ring");
 constexpr uint32_t kQBytes = 8 * 512;            // hi and lo of eight rows, as fragments
-constexpr uint32_t kOffMerge = kRingBytes;
-constexpr uint32_t kOffQ = kOffMerge + kMergeBytes;
+constexpr uint32_t kOffQ = kRingBytes;
 constexpr uint32_t kOffSums = kOffQ + kQBytes;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   __shared__ __align__(8) uint32_t s_magic[2];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffSums);   // work before sequence i, n_seq + 1
-  float *merge = reinterpret_cast<float *>(smem + kOffMerge);
+  auto state_of = [&](uint32_t w) { return reinterpret_cast<float *>(smem + w * kStages * kUnitBytes); };
   const uint32_t ring = smem_addr(smem) + warp * kStages * kUnitBytes;
   const uint32_t bar0 = smem_addr(&bars[warp * kStages]);
 
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     float lsum = l.x + l.y;
     lsum += __shfl_xor_sync(0xffffffffu, lsum, 1);
     lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
-    float *mine = merge + warp * kMergeFloats;
+    float *mine = state_of(warp);
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -441,12 +441,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       float2 ml[kWarps];
 #pragma unroll
       for (uint32_t w = 0; w < kWarps; ++w) {
-        ml[w] = *reinterpret_cast<const float2 *>(merge + w * kMergeFloats + kRows * kMergeRow + 2 * mr);
+        ml[w] = *reinterpret_cast<const float2 *>(state_of(w) + kRows * kMergeRow + 2 * mr);
         M = fmaxf(M, ml[w].x);
       }
 #pragma unroll
       for (uint32_t w = 0; w < kWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4 *>(merge + w * kMergeFloats + mr * kMergeRow + 4 * mc);
+        const float4 x = *reinterpret_cast<const float4 *>(state_of(w) + mr * kMergeRow + 4 * mc);
         const float a = weight(ml[w].x, M);
         L += ml[w].y * a;
         O.x += x.x * a, O.y += x.y * a, O.z += x.z * a, O.w += x.w * a;
@@ -514,7 +514,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
         }
       }
     }
-    __syncthreads();       // the merge area and s_last are free again
+    // the rings are free again, for bulk copies behind these plain accesses
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
     at = stop;
   }
   pdl_wait();              // the launch ends no earlier than the one before it
