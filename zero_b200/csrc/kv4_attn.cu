@@ -324,28 +324,26 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       float2 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = make_float2(0.f, 0.f);
+      uint4 kw[4], kd[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 kw[2], kd[2];
+      for (int u = 0; u < 4; ++u) {
+        kw[u] = lds128(base0 + kKv4TileBytes * (u >> 1) + 512 * (u & 1) + 16 * lane);
+        kd[u] = lds128(base0 + kKv4TileBytes * (u >> 1) + kKv4Ks + 64 * (u & 1) + 16 * c);
+      }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          kw[u] = lds128(base0 + kKv4TileBytes * h + 512 * u + 16 * lane);
-          kd[u] = lds128(base0 + kKv4TileBytes * h + kKv4Ks + 64 * u + 16 * c);
-        }
+      for (int g = 0; g < 4; ++g) {
+        const uint4 qa = lds128(qs + 1024 * g), qb = lds128(qs + 1024 * g + 512);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint4 qa = lds128(qs + 1024 * g), qb = lds128(qs + 1024 * g + 512);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t w = g == 0 ? kw[u].x : g == 1 ? kw[u].y : g == 2 ? kw[u].z : kw[u].w, w8 = w >> 8;
-            const uint32_t dw = g == 0 ? kd[u].x : g == 1 ? kd[u].y : g == 2 ? kd[u].z : kd[u].w;
-            float sc[4];
-            mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, w & 0x000F000Fu, w & 0x00F000F0u);
-            mma16816(sc, qb.x, qb.y, qb.z, qb.w, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
-            const float2 t = add2_rn(add2_rn(make_float2(sc[0], sc[1]), make_float2(sc[2], sc[3])),
-                                     make_float2(bias[g], bias[g]));
-            v[2 * h + u] = fma2_rn(t, __half22float2(bits2h(dw)), v[2 * h + u]);
-          }
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t w = g == 0 ? kw[u].x : g == 1 ? kw[u].y : g == 2 ? kw[u].z : kw[u].w, w8 = w >> 8;
+          const uint32_t dw = g == 0 ? kd[u].x : g == 1 ? kd[u].y : g == 2 ? kd[u].z : kd[u].w;
+          float sc[4];
+          mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, w & 0x000F000Fu, w & 0x00F000F0u);
+          mma16816(sc, qb.x, qb.y, qb.z, qb.w, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+          float2 t = make_float2(sc[0], sc[1]);
+          if (kLo) t = add2_rn(t, make_float2(sc[2], sc[3]));
+          t = add2_rn(t, make_float2(bias[g], bias[g]));
+          v[u] = fma2_rn(t, __half22float2(bits2h(dw)), v[u]);
         }
       }
       float mx = m;
