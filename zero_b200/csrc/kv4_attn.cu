@@ -26,7 +26,12 @@
 //   Keys stay integers: a masked nibble is a subnormal binary16, n 2^-24 (16
 //   times that at bits 4..7, which the query's other half carries as 1 / 16),
 //   so a value pair costs one logical operation.  Each group of 32 dims has
-//   its own sum, sum_g d_g (sum_j q_j n_j - 8 sum_j q_j), scaled in f32.
+//   its own sum, sum_g d_g (sum_j q_j n_j - 8 sum_j q_j), scaled in f32.  The
+//   matrix unit aligns a subnormal's products by its exponent, not by its
+//   leading bit, so their sum keeps some 17 bits: enough for 16-bit rows.  For
+//   f32 rows the words become the normal numbers n - 8 and 16 (n - 8), exact,
+//   with one more operation a pair (error
+//   3e-7 of the result's norm, against 1.7e-6 with the integers).
 //   Values are made binary16 by the bits' place: under a fixed exponent a
 //   nibble is a constant plus n, and (16 + n) d - 24 d is one exact fma since
 //   24 d is exact; for 256 + n an add takes the constant off first.
@@ -283,15 +288,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
           make_uint4(h2bits(h0), h2bits(__floats2half2_rn(y.x - f0.x, y.y - f0.y)), h2bits(h1),
                      h2bits(__floats2half2_rn(y.z - f1.x, y.w - f1.y)));
       // - 8 sum q of each group, in the units of the products
-      float qsum = (y.x + y.y) + 16.f * (y.z + y.w);
+      if (!kLo) {
+        float qsum = (y.x + y.y) + 16.f * (y.z + y.w);
 #pragma unroll
-      for (int off = 1; off < 8; off <<= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
-      if ((lane & 7u) == 0) s_bias[warp][lane >> 3] = qsum * (-8.f * 0x1p-24f);
+        for (int off = 1; off < 8; off <<= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
+        if ((lane & 7u) == 0) s_bias[warp][lane >> 3] = qsum * (-8.f * 0x1p-24f);
+      }
       if (lane == 0) {
         // keys that the row sees: 0 .. limit - 1 (none when its position is negative)
         const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + qtok + 1;
         s_limit[warp] = pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
-        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + 24 - 8 + e) << 23);
+        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + (kLo ? 0 : 24) - 8 + e) << 23);
       }
     }
     __syncthreads();
@@ -303,7 +310,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
 
     float bias[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) bias[g] = s_bias[r][g];
+    for (int g = 0; g < 4; ++g) bias[g] = kLo ? 0.f : s_bias[r][g];
 
     // o[n]: dims 16 n + r (and + 8) of rows 2 c and 2 c + 1; m, l: row r
     float o[8][4], m = -INFINITY;
@@ -338,11 +345,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
           const uint32_t w = g == 0 ? kw[u].x : g == 1 ? kw[u].y : g == 2 ? kw[u].z : kw[u].w, w8 = w >> 8;
           const uint32_t dw = g == 0 ? kd[u].x : g == 1 ? kd[u].y : g == 2 ? kd[u].z : kd[u].w;
           float sc[4];
-          mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, w & 0x000F000Fu, w & 0x00F000F0u);
-          mma16816(sc, qb.x, qb.y, qb.z, qb.w, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+          uint32_t n[4] = {w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
+          if (kLo) {    // 1024 + n, less 1032; 1024 + 16 n, less 1152
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              n[x] = h2bits(__hsub2(bits2h(n[x] | 0x64006400u), bits2h(x & 1 ? 0x64806480u : 0x64086408u)));
+          }
+          mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, n[0], n[1]);
+          mma16816(sc, qb.x, qb.y, qb.z, qb.w, n[2], n[3]);
           float2 t = make_float2(sc[0], sc[1]);
-          if (kLo) t = add2_rn(t, make_float2(sc[2], sc[3]));
-          t = add2_rn(t, make_float2(bias[g], bias[g]));
+          t = add2_rn(t, kLo ? make_float2(sc[2], sc[3]) : make_float2(bias[g], bias[g]));
           v[u] = fma2_rn(t, __half22float2(bits2h(dw)), v[u]);
         }
       }

@@ -457,10 +457,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             const uint64_t b = op_desc + slot * (kOpBytes >> 4);
             if (elect_one()) {
 #pragma unroll
-              for (uint32_t kk = 0; kk < 8; ++kk)
+              for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
 #pragma unroll
-                for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
-                  umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * part, b + 16 * kk, kIdesc, t >= 4 || kk || part);
+                for (uint32_t kk = 0; kk < 8; ++kk)
+                  umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * (kLo ? 1 - part : 0), b + 16 * kk, kIdesc, t >= 4 || kk || part);
               if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
               if (t >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
             }
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
               for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
 #pragma unroll
                 for (uint32_t kk = 0; kk < 8; ++kk)
-                  umma_f16_ss(sc, a0 + part * (kOpBytes >> 4) + 16 * kk, b + 16 * kk, kIdesc, part || kk);
+                  umma_f16_ss(sc, a0 + (kLo ? 1 - part : 0) * (kOpBytes >> 4) + 16 * kk, b + 16 * kk, kIdesc, part || kk);
               umma_commit(smem_addr(&bars.sfull[i]));
               if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
               if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
