@@ -600,6 +600,18 @@ def test_calls_leave_the_current_device_and_null_rows_alone(ctx):
     kv.close()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,nq", [
+    (2, 2, [31, 32, 33]), (6, 2, [10, 11, 12]), (4, 1, [8, 9, 1]), (16, 2, [4, 5, 3]), (16, 1, [2, 3, 0]), (11, 1, [3, 2, 3])])
+def test_attention_around_the_border_of_the_two_kernels(ctx, dtype, n_q, n_kv, nq):
+    """Up to 32 query rows per kv head, and more, in one call and in separate ones."""
+    c = make(ctx, n_q + n_kv, [nq[0] + 200, nq[1], nq[2] + 999], nq, n_q, n_kv, 32)
+    o, q = run_attn(c, dtype)
+    check_attn(c, o, q, dtype)
+    c["kv"].check()
+    c["kv"].close()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("n_seq,n", [(40, 100), (300, 20), (3, 1000)])
 def test_attention_many_short_pieces_per_cta(ctx, dtype, n_seq, n):
@@ -611,7 +623,7 @@ def test_attention_many_short_pieces_per_cta(ctx, dtype, n_seq, n):
     c["kv"].close()
 
 
-@pytest.mark.parametrize("nq", [1, 9])
+@pytest.mark.parametrize("nq", [1, 9, 20])
 def test_attention_of_the_most_sequences(ctx, nq):
     """1024 sequences, the largest table of sums; every 64th is checked."""
     lens = [nq + (i * 37) % 90 for i in range(1024)]

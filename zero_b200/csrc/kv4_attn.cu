@@ -4,7 +4,7 @@
 // own position: row i's queries are its last ones, query t of n at position
 // kv_len - n + t.
 //
-// kv4_rows_kernel: at most 16 query rows per kv head (decode, short
+// kv4_rows_kernel: at most 32 query rows per kv head (decode, short
 // continuations); kv4_prompt.cu takes the sequences with more.
 // Bound by the cache read, 144 bytes per key and kv head, and close behind it
 // by instruction issue: unpacking 256 values per key and head.
@@ -30,8 +30,8 @@
 //   matrix unit aligns a subnormal's products by its exponent, not by its
 //   leading bit, so their sum keeps some 17 bits: enough for 16-bit rows.  For
 //   f32 rows the words become the normal numbers n - 8 and 16 (n - 8), exact,
-//   with one more operation a pair (error
-//   3e-7 of the result's norm, against 1.7e-6 with the integers).
+//   with one more operation a pair (error 3e-7 of the result's norm, against
+//   1.7e-6 with the integers).
 //   Values are made binary16 by the bits' place: under a fixed exponent a
 //   nibble is a constant plus n, and (16 + n) d - 24 d is one exact fma since
 //   24 d is exact; for 256 + n an add takes the constant off first.

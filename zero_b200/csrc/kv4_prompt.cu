@@ -1,7 +1,7 @@
 // kv4_prompt.cu — attention of prompts and prompt chunks over the paged 4-bit
 // KV cache, on tcgen05.
 //
-// The same formula as kv4_attn.cu for sequences with more than 16 query rows
+// The same formula as kv4_attn.cu for sequences with more than 32 query rows
 // per kv head.  Bound by the tensor cores (4 * 128 flops per query head and
 // key, twice that for f32 rows) and, as closely, by the exponentials: 128 x
 // 128 scores are 1024 cycles of either.

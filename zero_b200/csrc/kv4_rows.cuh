@@ -93,7 +93,17 @@ __device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, co
   v[3] = h2bits(__hfma2(bits2h((x & 0x03C003C0u) | g.x16), d, m24d));
 }
 
-// Query rows per kv head above which a sequence goes to the prompt kernel.
-constexpr uint32_t kKv4FewRows = 16;
+// Query rows per kv head above which a sequence goes to the prompt kernel
+// (kv4_prompt.cu), whose time hardly depends on the rows of a tile, while
+// kv4_attn.cu's grows with every eighth.  Eight kv heads, group of four, us:
+//                        16 rows      32 rows      48 rows      64 rows
+//                      few  prompt  few  prompt  few  prompt  few  prompt
+//   f32  16 x  4096    51.5  84.4   89.5  85.4  127.6  86.8  166.5  87.3
+//         1 x 65536    49.4  94.6   84.3  95.9  120.0  97.2  155.9  97.5
+//         1 x   700    10.5  24.8   12.5  25.1   12.5  26.2   12.7  26.8
+//   f16  16 x  4096    43.9  97.5   75.6  98.5  107.0  99.0  139.0  99.6
+//        64 x   700    43.3  93.0   75.2  94.8  106.8  95.1  137.8  95.9
+//         1 x 65536    42.6 121.9   70.5 122.9   99.6 123.7  128.9 123.9
+constexpr uint32_t kKv4FewRows = 32;
 
 }  // namespace zgpu
