@@ -195,23 +195,28 @@ __global__ void __launch_bounds__(kReleaseThreads) kv4_release_kernel(const Kv4R
 
 // -------------------------------------------------------- append / gather
 template <class T>
-__device__ __forceinline__ float4 load4(const T *p);
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]);
 template <>
-__device__ __forceinline__ float4 load4<float>(const float *p) {
-  return *reinterpret_cast<const float4 *>(p);
+__device__ __forceinline__ void load8<float>(const float *p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 template <>
-__device__ __forceinline__ float4 load4<__half>(const __half *p) {
-  const uint2 u = *reinterpret_cast<const uint2 *>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ void load8<__half>(const __half *p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+    x[2 * e] = f.x, x[2 * e + 1] = f.y;
+  }
 }
 template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16 *p) {
-  const uint2 u = *reinterpret_cast<const uint2 *>(p);
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xFFFF0000u));
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
 }
 __device__ __forceinline__ void store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
 __device__ __forceinline__ void store4(__half *p, float4 v) {
@@ -221,13 +226,6 @@ __device__ __forceinline__ void store4(__half *p, float4 v) {
 __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v) {
   __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
   *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
-}
-
-// The larger magnitude, NaN if either is.
-__device__ __forceinline__ float max_abs_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
-  return r;
 }
 
 // n = q + 8 of one value where the quick rounding of x / d cannot be trusted:
@@ -245,46 +243,73 @@ __device__ __forceinline__ uint32_t nibble_exact(float x, float d, float inv) {
   return static_cast<uint32_t>(static_cast<int>(r) + 8);
 }
 
-// One row of 128 values, four per lane, eight lanes per group: the lane's four
-// n and the group's scale.  A group that cannot be held (a non-finite value, a
-// magnitude above 8 * 2720) is stored as zeros and recorded as a numerical
-// error.  The work is bound by instruction issue, so the common case is kept
-// short: x / d is rounded by adding 1.5 * 2^23, and only a warp in which some
-// remainder reaches d / 2 (a tie, or a quotient rounded onto a border) takes
-// the exact form.
-__device__ __forceinline__ void quantise4(float4 v, uint32_t lane, uint32_t (&n)[4], __half *scale, uint32_t *status) {
-  const float x[4] = {v.x, v.y, v.z, v.w};
-  float amax = max_abs_nan(max_abs_nan(x[0], x[1]), max_abs_nan(x[2], x[3]));
+// Eight values of a row a lane, four lanes a group: the lane's n, the even
+// dims' at bits 4 s of the low half and the odd dims' of the high half, and the
+// group's scale.  A group that cannot be held (a non-finite value, a magnitude
+// above 8 * 2720) is stored as zeros and recorded as a numerical error.  The
+// work is bound by instruction issue, so the common case is kept short: the
+// sign of the group's largest magnitude comes from its maximum and minimum,
+// and only a warp in which the two are of one magnitude looks for the first;
+// x / d is rounded by adding 1.5 * 2^23, and only a warp in which some
+// remainder reaches d / 2 (a tie, or a quotient rounded onto a border), or some
+// scale is subnormal (a quotient may then be far outside -8..8), takes the
+// exact form.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t lane, __half *scale, uint32_t *status) {
+  float mx, mn = fminf(fminf(fminf(x[0], x[1]), x[2]), fminf(fminf(x[3], x[4]), x[5]));
+  mn = fminf(fminf(mn, x[6]), x[7]);
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(mx) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(x[3]), "f"(x[4]));
+  asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(x[5]), "f"(x[6]));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(x[7]));
 #pragma unroll
-  for (int off = 1; off < 8; off <<= 1) amax = max_abs_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  // the sign of the first value of that magnitude
-  const bool has[4] = {fabsf(x[0]) == amax, fabsf(x[1]) == amax, fabsf(x[2]) == amax, fabsf(x[3]) == amax};
-  const float mine = has[0] ? x[0] : has[1] ? x[1] : has[2] ? x[2] : x[3];
-  const uint32_t any = __ballot_sync(0xffffffffu, has[0] || has[1] || has[2] || has[3]);
-  const uint32_t below = __ballot_sync(0xffffffffu, mine < 0.f), group = 0xFFu << (lane & 24u);
-  const uint32_t first = any & group & (0u - (any & group));     // the group's lowest lane that has it
-  float d = (first & below ? 0.125f : -0.125f) * amax;
+  for (int off = 1; off < 4; off <<= 1) {
+    const float a = __shfl_xor_sync(0xffffffffu, mx, off);
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(a));
+  }
+  float amax;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(mx), "f"(-mn));
+  bool neg = -mn > mx;
+  if (__any_sync(0xffffffffu, mx == -mn && mx > 0.f)) {
+    float mine = 0.f;      // the lane's first value of that magnitude
+#pragma unroll
+    for (int e = 7; e >= 0; --e) mine = fabsf(x[e]) == amax ? x[e] : mine;
+    const uint32_t any = __ballot_sync(0xffffffffu, mine != 0.f) & (0xFu << (lane & 28u));
+    const uint32_t below = __ballot_sync(0xffffffffu, mine < 0.f);
+    neg = any & (0u - any) & below;                                // the group's lowest lane that has it
+  }
+  float d = (neg ? 0.125f : -0.125f) * amax;
   __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(d)));
   d = __half2float(dh);
   if (!(fabsf(d) <= kKv4MaxScale) || !(amax < INFINITY)) {
-    if ((lane & 7u) == 0) atomicOr(status, ZDEV_ERR_NUMERICAL);
+    if ((lane & 3u) == 0) atomicOr(status, ZDEV_ERR_NUMERICAL);
     d = 0.f;
     dh = __float2half_rn(0.f);
   }
   *scale = dh;
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+  constexpr float kAdd = 12582912.f + 8.f;     // its last four bits are n
   float worst = 0.f;
+  uint32_t n[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float t = fmaf(x[e], inv, 12582912.f), r = t - 12582912.f;
-    worst = fmaxf(worst, fabsf(fmaf(-r, d, x[e])));
-    n[e] = __vimin_s32_relu(__float_as_int(t) - (0x4B400000 - 8), 15);   // 0..15: a tiny scale may be far from m / 8
+  for (int e = 0; e < 8; e += 2) {
+    const float2 v = make_float2(x[e], x[e + 1]);
+    const float2 t = fma2_rn(v, make_float2(inv, inv), make_float2(kAdd, kAdd));
+    const float2 r = add2_rn(make_float2(kAdd, kAdd), make_float2(-t.x, -t.y));
+    const float2 left = fma2_rn(r, make_float2(d, d), v);
+    worst = fmaxf(fmaxf(worst, fabsf(left.x)), fabsf(left.y));
+    n[e] = __float_as_uint(fminf(t.x, kAdd + 7.f));
+    n[e + 1] = __float_as_uint(fminf(t.y, kAdd + 7.f));
   }
-  if (__any_sync(0xffffffffu, !(worst < 0.5f * fabsf(d)))) {
+  if (__any_sync(0xffffffffu, !(worst < (fabsf(d) < 0x1p-14f ? 0.f : 0.5f * fabsf(d))))) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) n[e] = d != 0.f ? nibble_exact(x[e], d, inv) : 8u;
+    for (int e = 0; e < 8; ++e) n[e] = d != 0.f ? nibble_exact(x[e], d, inv) : 8u;
   }
+  uint32_t w = __byte_perm(n[0], n[1], 0x5410u);
+#pragma unroll
+  for (int e = 2; e < 8; e += 2) w += __byte_perm(n[e], n[e + 1], 0x5410u) << (2 * e);
+  return w;
 }
 
 // A 4 x 4 transpose of nibbles over the four lanes of this lane's parity in
@@ -317,28 +342,42 @@ __device__ __forceinline__ uint32_t scale_off(uint32_t t, uint32_t g) {
 
 constexpr uint32_t kRowWarps = 8;
 
-// A warp per (token, kv head): rows in with 512-byte loads, 144 bytes out.
+// A warp per (token, kv head): lanes 0..15 take the K row, 16..31 the V row,
+// lane 4 g + c of a half its dims 32 g + 8 c + 0..7.
+// Bound by instruction issue, close above the reads of the rows: 16384 tokens
+// of 8 kv heads in f32 take 37.6 us (134 MB in, 19 MB out, 4.1 TB/s), 203
+// instructions a warp and row pair at 72 % issue.  Four values of both rows a
+// lane took 47 us: the group's maximum, scale and sign cost as much for four
+// values as for eight.  Four CTAs fit an SM at 57 registers; bounds for five and
+// six, at the price of the values on their way, measured 40 and 49 us.
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
   // the number of warps is a multiple of n_kv: a warp keeps its head
   const uint32_t lane = threadIdx.x & 31, w0 = blockIdx.x * kRowWarps + (threadIdx.x >> 5), head = w0 % p.n_kv;
-  const uint32_t step = gridDim.x * kRowWarps / p.n_kv;
+  const uint32_t step = gridDim.x * kRowWarps / p.n_kv, c = lane & 3u, g = (lane >> 2) & 3u;
+  const bool is_v = lane >= 16;
   uint32_t token = w0 / p.n_kv;
   if (token >= p.n_tokens) return;
-  const T *kp = static_cast<const T *>(p.k) + head * kKv4Head + 4 * lane;
-  const T *vp = static_cast<const T *>(p.v) + head * kKv4Head + 4 * lane;
+  const T *rows = static_cast<const T *>(is_v ? p.v : p.k) + head * kKv4Head + 8 * (lane & 15u);
+  const uint64_t stride = is_v ? p.v_stride : p.k_stride;
+  // V: the lane's pieces of a token are dims r and r + 2 of each eight
+  const uint32_t r = 4 * (c & 1u) + (c >> 1);
+  const uint32_t lane_off = is_v ? kKv4V + 64 * r + 4 * g : 16 * c + 4 * g;
+  const uint32_t scale_off0 = (is_v ? kKv4Vs : kKv4Ks) + 4 * g;
   uint32_t next_slot = p.slots[token];
-  float4 next_k = load4(kp + token * p.k_stride), next_v = load4(vp + token * p.v_stride);
+  float next[8];
+  load8(rows + token * stride, next);
   while (true) {
     const uint32_t slot = next_slot;
-    const float4 kx = next_k, vx = next_v;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = next[e];
     // the next token's rows are on their way while this one's are worked on
     const bool more = p.n_tokens - token > step;
     token += step;
     if (more) {
       next_slot = p.slots[token];
-      next_k = load4(kp + token * p.k_stride);
-      next_v = load4(vp + token * p.v_stride);
+      load8(rows + token * stride, next);
     }
     if (slot >= p.n_slots) {
       if (slot != kKv4NoSlot && lane == 0) atomicOr(p.status, ZDEV_ERR_BOUNDS);
@@ -346,26 +385,35 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
       continue;
     }
     uint8_t *tile = p.pool + kv4_tile_off(slot, head, p.n_kv, p.bt_log2);
-    const uint32_t t = slot % kKv4Tile;
-    __half ks, vs;
-    uint32_t kn[4], vn[4];
-    quantise4(kx, lane, kn, &ks, p.status);
-    quantise4(vx, lane, vn, &vs, p.status);
-    // two lanes make a K word: dims 0, 2 | 1, 3 of the one, 4, 6 | 5, 7 of the other
-    uint32_t w = kn[0] | kn[2] << 4 | kn[1] << 16 | kn[3] << 20;
-    if (lane & 1u) w <<= 8;
-    w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    const uint32_t vt = transpose_nibbles(vn[0] | vn[1] << 4 | vn[2] << 8 | vn[3] << 12, lane);
-    if (!(lane & 1u)) *reinterpret_cast<uint32_t *>(tile + k_off(t, lane)) = w;
-    *reinterpret_cast<uint16_t *>(tile + v_off(t, lane)) = static_cast<uint16_t>(kv4_v_bits(vt));
-    if ((lane & 7u) == 0) {
-      *reinterpret_cast<__half *>(tile + kKv4Ks + scale_off(t, lane / 8)) = ks;
-      *reinterpret_cast<__half *>(tile + kKv4Vs + scale_off(t, lane / 8)) = vs;
+    const uint32_t t = slot % kKv4Tile, half = t >> 3, at = 16 * ((t >> 1) & 3u) + 2 * (t & 1u);
+    __half scale;
+    const uint32_t w = quantise8(x, lane, &scale, p.status);
+    // V: a 4 x 4 transpose of bytes over the group's lanes, after which byte s
+    // holds dims 8 s + r and 8 s + r + 2 in its low and high four bits
+    uint32_t q = __shfl_xor_sync(0xffffffffu, w, 2);
+    uint32_t v = __byte_perm(w, q, c & 2u ? 0x3276u : 0x5410u);
+    q = __shfl_xor_sync(0xffffffffu, v, 1);
+    v = __byte_perm(v, q, c & 1u ? 0x3715u : 0x6240u);
+    if (is_v) {
+      const uint32_t lo = v & 0x0F0F0F0Fu, hi = (v >> 4) & 0x0F0F0F0Fu;
+      const uint32_t s3 = __byte_perm(lo, hi, 0x0703u) & 0x000F000Fu;
+      const uint32_t both = (__byte_perm(lo, hi, 0x0400u) & 0x000F000Fu) << 6 | (__byte_perm(lo, hi, 0x0501u) & 0x000F000Fu) << 2 |
+                            (__byte_perm(lo, hi, 0x0602u) & 0x000F000Fu) << 10 | (s3 & 0x00030003u) << 14 |
+                            ((s3 >> 2) & 0x00030003u);
+      uint8_t *to = tile + lane_off + 512 * half + at;
+      *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(both);
+      *reinterpret_cast<uint16_t *>(to + 128) = static_cast<uint16_t>(both >> 16);
+    } else {
+      *reinterpret_cast<uint32_t *>(tile + lane_off + 64 * t) = w;
     }
+    if (c == 0) *reinterpret_cast<__half *>(tile + scale_off0 + 64 * half + at) = scale;
     if (!more) return;
   }
 }
 
+// A warp per (token, kv head), four values of both rows a lane, so that a store
+// is 512 contiguous bytes.  Bound by the writes: 16384 tokens of 8 kv heads to f32
+// take 29.5 us (134 MB out, 19 MB in, 5.2 TB/s).
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4RowsParams p) {
   // the number of warps is a multiple of n_kv: a warp keeps its head

@@ -55,10 +55,7 @@ __host__ __device__ inline size_t kv4_tile_off(uint32_t slot, uint32_t head, uin
   return (((static_cast<size_t>(block) * n_kv + head) << (bt_log2 - 4)) + tile) * kKv4TileBytes;
 }
 
-// A token's 16 bits of V from nibbles s at bits 4 s, and back.
-__host__ __device__ inline uint32_t kv4_v_bits(uint32_t n) {
-  return (n & 15u) << 6 | ((n >> 4) & 15u) << 2 | ((n >> 8) & 15u) << 10 | ((n >> 12) & 3u) << 14 | (n >> 14);
-}
+// The nibbles s of a token's 16 bits of V, at bits 4 s.
 __host__ __device__ inline uint32_t kv4_v_nibbles(uint32_t v) {
   return ((v >> 6) & 15u) | ((v >> 2) & 15u) << 4 | ((v >> 10) & 15u) << 8 | ((v >> 14) | (v & 3u) << 2) << 12;
 }
