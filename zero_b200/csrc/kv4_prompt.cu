@@ -62,8 +62,10 @@ constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemCols = 512;
 constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 // Operand tiles: [row / 8][16-byte chunk][row % 8][16 bytes]
 constexpr uint32_t kLbo = 128, kSbo = 2048;
+constexpr uint32_t kPieces = 4;                       // pieces made known ahead
 
 struct Bars {
+  uint64_t nfull[kPieces], nempty[kPieces];
   uint64_t qfull, qempty, rfull[2][kRawStages], rempty[2][kRawStages], full[kSlots], empty[kSlots];
   uint64_t sfull[2], pfull[2], ofull[2], oempty[2], join, drain;
 };
@@ -128,14 +130,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t &bar, uint32_t parity, uint32
   return __all_sync(0xffffffffu, wait(bar, parity, status));
 }
 
-// Walks the pieces of a range; every warp walks for itself.  A piece of n key
-// tiles is n + kPieceCost units of work, the tiles being the last n.
+// A piece of work, as the loading warp makes it known to the others: code that
+// runs once a piece comes from behind the instruction cache (some 16 cycles an
+// instruction), so one warp walks, ahead of the rest, and they read.
 struct Piece {
   uint32_t seq, head, rt;        // what
-  uint32_t t0, t1, n;            // key tiles t0 .. t1 - 1 of n
+  uint32_t t0, t1, n;            // key tiles t0 .. t1 - 1 of n; t1 = 0 ends the range
   Kv4Seq s;
-  uint64_t at;                   // the piece's first tile in units of work
+  uint32_t c0, c1;               // the ranges that share the piece
 };
+
+// Walks the pieces of a range.  A piece of n key tiles is n + kPieceCost units
+// of work, the tiles being the last n.
 
 template <uint32_t MR>
 struct Walk {
@@ -143,7 +149,8 @@ struct Walk {
   const uint32_t *lens, *nqs, *q0s;
   uint32_t n_kv, group;
   uint64_t at, end;
-  Piece p;
+  Piece p = {};
+  uint64_t first = 0;            // the piece's first tile in units of work
   uint32_t n_rt, off;            // units of the piece before `at`
   bool fresh;
 
@@ -165,7 +172,7 @@ struct Walk {
     n_rt = row_tiles(p.s.nq, group);
   }
   // The first piece: all lanes of the warp take part.
-  __device__ __noinline__ void start(uint32_t n_seq) {
+  __device__ __forceinline__ void start(uint32_t n_seq) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t lo = 0, hi = n_seq;
     while (hi - lo > 1) {
@@ -200,7 +207,7 @@ struct Walk {
     fresh = true;
   }
   // The next piece of the range with a key tile in it, or false.
-  __device__ __noinline__ bool next() {
+  __device__ __forceinline__ bool next() {
     while (at < end) {
       if (!fresh) {
         off = 0;
@@ -219,7 +226,7 @@ struct Walk {
         }
       }
       fresh = false;
-      p.at = at - off + kPieceCost;
+      first = at - off + kPieceCost;
       const uint64_t left = end - at;
       const uint32_t last = left < p.n + kPieceCost - off ? off + static_cast<uint32_t>(left) : p.n + kPieceCost;
       p.t0 = off > kPieceCost ? off - kPieceCost : 0u;
@@ -235,84 +242,91 @@ struct Walk {
 // (hi and lo for f32) in the operand layout, and each row's factor of the
 // scores.  Eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
 // kq + 12 of row kr: the eight lanes of a 16-byte store phase write 128
-// contiguous bytes.  f32 and bf16 rows are scaled by a power of two (the
-// largest value in [1, 2)) to fit binary16's range; f16 rows are copied.
+// contiguous bytes.  All of a warp's rows are on their way at once, copied to
+// where they end up (an f32 chunk's two halves to its hi and its lo place);
+// then f32 and bf16 rows are scaled by a power of two (the largest value in
+// [1, 2)) to fit binary16's range, in place, each lane its own chunks.
 template <class T>
-__device__ __noinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
-                                          uint32_t share) {
+__device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
+                                             uint32_t share) {
   constexpr bool kLo = sizeof(T) == 4, kCopy = __is_same(T, __half);
-  constexpr uint32_t MR = kLo ? 128 : 256, kVec = kLo ? 8 : 4, kBatch = kLo ? 2 : 3, kShares = kConvWarps + kQWarps;
+  constexpr uint32_t MR = kLo ? 128 : 256, kShares = kConvWarps + kQWarps;
   const uint32_t lane = threadIdx.x & 31, kr = lane & 7, kq = lane >> 3, n_rows = pc.s.nq * p.group;
-  const uint32_t seq_q0 = pc.s.q0, head = pc.head, row0 = pc.rt * MR;
+  const uint32_t row0 = pc.rt * MR, at = smem_addr(q_op) + 16 * kr + kLbo * kq;
+  const T *q = static_cast<const T *>(p.q) + pc.s.q0 * p.q_stride + static_cast<size_t>(pc.head) * p.group * kKv4Head + 8 * kq;
 #pragma unroll 1
-  for (uint32_t g0 = share; g0 < MR / 8; g0 += kShares * kBatch) {
-    uint4 raw[kBatch][kVec];
+  for (uint32_t g = share; g < MR / 8; g += kShares) {
+    const uint32_t row = row0 + 8 * g + kr, tok = row / p.group, hd = row - tok * p.group;
+    const bool is = row < n_rows;       // zeros behind the last row
+    const T *src = is ? q + tok * p.q_stride + hd * kKv4Head : static_cast<const T *>(p.q);
 #pragma unroll
-    for (uint32_t j = 0; j < kBatch; ++j) {
-      const uint32_t g = g0 + kShares * j, row = row0 + 8 * g + kr, tok = row / p.group, hd = row % p.group;
-      const T *qp = static_cast<const T *>(p.q) + (seq_q0 + static_cast<uint64_t>(tok)) * p.q_stride +
-                    (static_cast<size_t>(head) * p.group + hd) * kKv4Head + 8 * kq;
-#pragma unroll
-      for (uint32_t k = 0; k < kVec; ++k)
-        raw[j][k] = g < MR / 8 && row < n_rows ? __ldg(reinterpret_cast<const uint4 *>(qp + (kLo ? 32 * (k / 2) + 4 * (k & 1) : 32 * k)))
-                                               : make_uint4(0u, 0u, 0u, 0u);
+    for (uint32_t k = 0; k < 4; ++k) {
+      cp_async16(at + kSbo * g + 4 * kLbo * k, src + (is ? 32 * k : 0), is ? 16u : 0u);
+      if (kLo) cp_async16(at + kOpBytes + kSbo * g + 4 * kLbo * k, src + (is ? 32 * k + 4 : 0), is ? 16u : 0u);
     }
+    if (kCopy && kq == 0) s_scl[8 * g + kr] = p.scale * 1.44269504088896341f;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!kCopy) {
+#pragma unroll 1
+    for (uint32_t g = share; g < MR / 8; g += kShares) {
+      uint8_t *dst = q_op + kSbo * g + 16 * kr + kLbo * kq;
+      uint4 a[4], b[4];
 #pragma unroll
-    for (uint32_t j = 0; j < kBatch; ++j) {
-      const uint32_t g = g0 + kShares * j;
-      if (g >= MR / 8) break;
-      uint8_t *dst = q_op + kSbo * g + 16 * kr;
-      int e = 0;
-      if (!kCopy) {
-        float amax = 0.f;
-        if (kLo) {
-#pragma unroll
-          for (uint32_t k = 0; k < kVec; ++k)
-            amax = fmaxf(fmaxf(fmaxf(fabsf(__uint_as_float(raw[j][k].x)), fabsf(__uint_as_float(raw[j][k].y))),
-                               fmaxf(fabsf(__uint_as_float(raw[j][k].z)), fabsf(__uint_as_float(raw[j][k].w)))), amax);
-        } else {
-          __nv_bfloat162 mx = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-          for (uint32_t k = 0; k < kVec; ++k) {
-            const uint32_t u[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) mx = __hmax2(mx, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&u[x])));
-          }
-          amax = fmaxf(__low2float(mx), __high2float(mx));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-        e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-        e = e < -100 ? -100 : e > 110 ? 110 : e;
+      for (int k = 0; k < 4; ++k) {
+        a[k] = *reinterpret_cast<const uint4 *>(dst + 4 * kLbo * k);
+        if (kLo) b[k] = *reinterpret_cast<const uint4 *>(dst + kOpBytes + 4 * kLbo * k);
       }
+      float amax = 0.f;
+      if (kLo) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          amax = fmaxf(fmaxf(fmaxf(fabsf(__uint_as_float(a[k].x)), fabsf(__uint_as_float(a[k].y))),
+                             fmaxf(fabsf(__uint_as_float(a[k].z)), fabsf(__uint_as_float(a[k].w)))), amax);
+          amax = fmaxf(fmaxf(fmaxf(fabsf(__uint_as_float(b[k].x)), fabsf(__uint_as_float(b[k].y))),
+                             fmaxf(fabsf(__uint_as_float(b[k].z)), fabsf(__uint_as_float(b[k].w)))), amax);
+        }
+      } else {
+        __nv_bfloat162 mx = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u[4] = {a[k].x, a[k].y, a[k].z, a[k].w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx = __hmax2(mx, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&u[x])));
+        }
+        amax = fmaxf(__low2float(mx), __high2float(mx));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+      int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+      e = e < -100 ? -100 : e > 110 ? 110 : e;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       if (kq == 0)
         s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t hi[4] = {raw[j][kCopy ? k : 0].x, raw[j][kCopy ? k : 0].y, raw[j][kCopy ? k : 0].z, raw[j][kCopy ? k : 0].w}, lo[4];
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int x = 0; x < (kCopy ? 0 : 4); ++x) {
+        for (int x = 0; x < 4; ++x) {
           float2 f;
           if (kLo) {
-            const uint4 u = raw[j][kLo ? 2 * k + (x >> 1) : 0];
+            const uint4 u = x < 2 ? a[k] : b[k];
             f = x & 1 ? make_float2(__uint_as_float(u.z), __uint_as_float(u.w))
                       : make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
           } else {
-            const uint4 u = raw[j][k];
-            const uint32_t w = x == 0 ? u.x : x == 1 ? u.y : x == 2 ? u.z : u.w;
+            const uint32_t w = x == 0 ? a[k].x : x == 1 ? a[k].y : x == 2 ? a[k].z : a[k].w;
             f = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
           }
           f = mul2_rn(f, make_float2(down, down));
           const __half2 h = __floats2half2_rn(f.x, f.y);
           hi[x] = h2bits(h);
           if (kLo) {
-            const float2 b = __half22float2(h);
-            lo[x] = h2bits(__floats2half2_rn(f.x - b.x, f.y - b.y));
+            const float2 r = __half22float2(h);
+            lo[x] = h2bits(__floats2half2_rn(f.x - r.x, f.y - r.y));
           }
         }
-        *reinterpret_cast<uint4 *>(dst + kLbo * (kq + 4 * k)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + kLbo * (kq + 4 * k)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4 *>(dst + 4 * kLbo * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (kLo) *reinterpret_cast<uint4 *>(dst + kOpBytes + 4 * kLbo * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
   }
@@ -329,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
   constexpr float kPShift = kLo ? 15.f : 7.f, kLazy = kLo ? 0.f : 8.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) Bars bars;
+  __shared__ Piece s_piece[kPieces];
   __shared__ uint32_t tmem_base, s_last;
   __shared__ float s_scl[kMaxRows];
   __shared__ float s_ml[2][2][128][2];
@@ -349,6 +364,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
+    for (uint32_t i = 0; i < kPieces; ++i) {
+      mbar_init(smem_addr(&bars.nfull[i]), 1);
+      mbar_init(smem_addr(&bars.nempty[i]), kThreads / 32 - 1);
+    }
     mbar_init(smem_addr(&bars.qfull), kQWarps + kConvWarps);
     mbar_init(smem_addr(&bars.qempty), 1 + kSoftWarps);     // the last S, and every reader of s_scl
     for (int i = 0; i < 2; ++i) {
@@ -412,12 +431,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
   if (G > gridDim.x) G = gridDim.x;
 
   if (blockIdx.x < G) {
-    Walk<MR> walk;
-    walk.sums = sums, walk.lens = lens, walk.nqs = nqs, walk.q0s = q0s;
-    walk.n_kv = p.n_kv, walk.group = p.group;
-    walk.at = W * blockIdx.x / G;
-    walk.end = W * (blockIdx.x + 1) / G;
-    walk.start(p.n_seq);
     // steps of a piece with key tiles 0 .. n - 1: stream t & 1, key tile kv_of(t)
     auto steps = [](uint32_t n) { return kLo ? n : 2 * n; };
     // The place of key tile j and of its values in the ring's order.  f32 rows
@@ -427,6 +440,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     auto key_tile = [](uint32_t j) { return kLo ? (j < 2 ? j : 2 * j - 1) : 2 * j; };
     auto value_tile = [](uint32_t j) { return kLo ? 2 * j + 2 : 2 * j + 1; };
     bool ok = true;
+    // The range's next piece, for every warp but the loading one.
+    uint32_t pieces = 0;
+    Piece pc;
+    auto next_piece = [&]() -> bool {
+      const uint32_t slot = pieces % kPieces;
+      ok = warp_wait(bars.nfull[slot], (pieces / kPieces) & 1, p.status);
+      if (!ok) return false;
+      ++pieces;
+      pc = s_piece[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&bars.nempty[slot]));
+      return pc.t1 != 0;
+    };
 
     if (warp == kMmaWarp) {
       // ------------------------------------------------------- MMA issuer
@@ -435,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
       const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
       const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
-      while (ok && walk.next()) {
-        const uint32_t n = walk.p.t1 - walk.p.t0, n_steps = steps(n);
+      while (ok && next_piece()) {
+        const uint32_t n = pc.t1 - pc.t0, n_steps = steps(n);
         ok = warp_wait(bars.qfull, item & 1, p.status);
         // S(0), S(1), then PV(t - 2) and S(t)
         for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
@@ -499,8 +525,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // lane h < 8: keys 16 h .. of the tile, table entries a tile ahead
       const uint32_t tpb_log2 = p.bt_log2 - 4;
       uint32_t kc = 0, issued[2] = {0, 0};
-      while (ok && walk.next()) {
-        const Piece &pc = walk.p;
+      Walk<MR> walk;
+      walk.sums = sums, walk.lens = lens, walk.nqs = nqs, walk.q0s = q0s;
+      walk.n_kv = p.n_kv, walk.group = p.group;
+      walk.at = W * blockIdx.x / G;
+      walk.end = W * (blockIdx.x + 1) / G;
+      walk.start(p.n_seq);
+      for (bool more = true; ok && more; ++pieces) {
+        const uint32_t piece_slot = pieces % kPieces;
+        if (pieces >= kPieces) ok = warp_wait(bars.nempty[piece_slot], (pieces / kPieces - 1) & 1, p.status);
+        if (!ok) break;
+        more = walk.next();
+        pc = walk.p;
+        if (!more) pc.t0 = pc.t1 = 0;
+        const uint64_t last = walk.first + pc.n;
+        pc.c0 = static_cast<uint32_t>(((walk.first + 1) * G - 1) / W);
+        pc.c1 = static_cast<uint32_t>((last * G - 1) / W);
+        if (lane == 0) {
+          s_piece[piece_slot] = pc;
+          mbar_arrive(smem_addr(&bars.nfull[piece_slot]));
+        }
         const uint32_t *table = p.table + static_cast<size_t>(pc.seq) * p.table_width;
         auto entry = [&](uint32_t t) -> uint32_t {
           const uint32_t tile = 8 * t + lane;
@@ -537,9 +581,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     } else if (warp >= kQ0) {
       // -------------------------------------------------------- query rows
       uint32_t item = 0;
-      while (ok && walk.next()) {
+      while (ok && next_piece()) {
         ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
-        if (ok) load_queries<T>(p, walk.p, smem + kOffQ, s_scl, warp - kQ0);
+        if (ok) load_queries<T>(p, pc, smem + kOffQ, s_scl, warp - kQ0);
         if (ok && lane == 0) mbar_arrive(smem_addr(&bars.qfull));
         ++item;
       }
@@ -617,8 +661,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         return true;
       };
       uint32_t kc = 0, item = 0;
-      while (ok && walk.next()) {
-        const uint32_t n = walk.p.t1 - walk.p.t0;
+      while (ok && next_piece()) {
+        const uint32_t n = pc.t1 - pc.t0;
         for (uint32_t t = 0; ok && t < n; ++t, ++kc) {
           ok = keys(kc);
           if (ok && (!kLo || kc > 0) && !(!kLo && t == 0)) ok = values(kLo ? kc - 1 : kc);
@@ -627,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           if (ok && t == 0) {
             ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
             if (!ok) break;
-            load_queries<T>(p, walk.p, smem + kOffQ, s_scl, kQWarps + cw);
+            load_queries<T>(p, pc, smem + kOffQ, s_scl, kQWarps + cw);
             if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
             ++item;
             if (!kLo) ok = values(kc);
@@ -648,8 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         if (lane == 0) mbar_arrive(smem_addr(&bars.join));
         return warp_wait(bars.join, joins++ & 1, p.status);
       };
-      while (ok && walk.next()) {
-        const Piece &pc = walk.p;
+      while (ok && next_piece()) {
         const uint32_t n = pc.t1 - pc.t0, n_steps = steps(n), trow = kLo ? row : 128 * i + row;
         const uint32_t grow = pc.rt * MR + trow, n_rows = pc.s.nq * p.group;
         const uint32_t tok = grow / p.group;
@@ -823,8 +866,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           __threadfence();
           if (!(ok = join())) break;
           // the ranges that share the piece
-          const uint32_t c0 = static_cast<uint32_t>(((pc.at + 1) * G - 1) / W);
-          const uint32_t c1 = static_cast<uint32_t>(((pc.at + pc.n) * G - 1) / W);
+          const uint32_t c0 = pc.c0, c1 = pc.c1;
           if (tid == 0) {
             s_last = atomicAdd(&p.counters[c0], 1u) == c1 - c0;
             if (s_last) p.counters[c0] = 0;
