@@ -456,8 +456,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
 
     if (warp == kMmaWarp) {
       // ------------------------------------------------------- MMA issuer
-      // The whole warp waits and counts; one elected lane issues.
-      uint32_t item = 0, kc0 = 0, sp[2] = {0, 0}, oc[2] = {0, 0};
+      // The whole warp waits and counts; one elected lane issues.  The streams
+      // wait on each other here, so the loop is kept short: places in the ring
+      // are counted on, what a step needs is looked for at once, and PV and S go
+      // out together.
+      uint32_t item = 0, oc[2] = {0, 0}, p_parity[2] = {0, 0};
+      // the next tile of keys and of values in the ring: place and phase
+      uint32_t k_slot = 0, k_phase = 0, v_slot = kLo ? 2 : 1, v_phase = 0;
+      bool first_key = kLo;
+      auto two_on = [](uint32_t &slot, uint32_t &phase) {
+        phase ^= slot != 0;
+        slot = slot ? slot - 1 : 2;
+      };
+      static_assert(kSlots == 3, "two_on");
       // operand descriptors: 16 more per K step of 16 (two 128-byte chunks)
       const uint64_t q_desc = umma_desc(smem_addr(smem) + kOffQ, kLbo, kSbo);
       const uint64_t op_desc = umma_desc(smem_addr(smem) + kOffOp, kLbo, kSbo);
@@ -467,53 +478,55 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         // S(0), S(1), then PV(t - 2) and S(t)
         for (uint32_t t = 0; ok && t < n_steps + 2; ++t) {
           const uint32_t i = t & 1, d = tmem + kTmemO + 128 * i, sc = tmem + kTmemS + 128 * i;
-          if (t >= 2 && t - 2 < n_steps) {
-            const uint32_t x = value_tile(kc0 + (kLo ? t - 2 : (t - 2) >> 1)), slot = x % kSlots;
-            if (kLo || i == 0) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
-            if (ok && t < 4 && oc[i] > 0) ok = warp_wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
-            // the next S's keys are looked for before P, so that S follows PV at once
-            if (ok && (kLo || i == 0) && t < n_steps) {
-              const uint32_t xk = key_tile(kc0 + (kLo ? t : t >> 1));
-              ok = warp_wait(bars.full[xk % kSlots], (xk / kSlots) & 1, p.status);
-            }
-            if (ok) ok = warp_wait(bars.pfull[i], sp[i] & 1, p.status);
-            ++sp[i];
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t b = op_desc + slot * (kOpBytes >> 4);
-            if (elect_one()) {
+          const bool pv = t >= 2, more = t < n_steps;     // PV(t - 2), S(t)
+          if (pv && t < 4 && oc[i] > 0) ok = warp_wait(bars.oempty[i], (oc[i] - 1) & 1, p.status);
+          // the next S's keys are looked for before P, so that S follows PV at once
+          const uint32_t v_bar = smem_addr(&bars.full[v_slot]), k_bar = smem_addr(&bars.full[k_slot]);
+          const uint32_t p_bar = smem_addr(&bars.pfull[i]), p_par = i ? p_parity[1] : p_parity[0];
+          const bool v_there = !pv || mbar_try_wait(v_bar, v_phase), k_there = !more || mbar_try_wait(k_bar, k_phase);
+          const bool p_there = !pv || mbar_try_wait(p_bar, p_par);
+          if (!__all_sync(0xffffffffu, v_there && k_there && p_there))
+            ok = ok && __all_sync(0xffffffffu, (!pv || slow_wait(v_bar, v_phase, p.status)) && (!more || slow_wait(k_bar, k_phase, p.status)) &&
+                                                   (!pv || slow_wait(p_bar, p_par, p.status)));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t bv = op_desc + v_slot * (kOpBytes >> 4), bk = op_desc + k_slot * (kOpBytes >> 4);
+          const uint64_t a0 = q_desc + (kLo ? 0 : i) * (kOpBytes >> 4);
+          const bool last = kLo || i == 1;                // the last stream to read the tiles
+          if (elect_one()) {
+            if (pv) {
 #pragma unroll
               for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
 #pragma unroll
                 for (uint32_t kk = 0; kk < 8; ++kk)
-                  umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * (kLo ? 1 - part : 0), b + 16 * kk, kIdesc, t >= 4 || kk || part);
-              if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
-              if (t >= n_steps) umma_commit(smem_addr(&bars.ofull[i]));
+                  umma_f16_ts(d, sc + 32 * (kk / 2) + 8 * (kk & 1) + 16 * (kLo ? 1 - part : 0), bv + 16 * kk, kIdesc, t >= 4 || kk || part);
+              if (!more) umma_commit(smem_addr(&bars.ofull[i]));
+              if (last) umma_commit(v_bar - smem_addr(&bars.full[0]) + smem_addr(&bars.empty[0]));
             }
-            __syncwarp();
-          }
-          if (t < n_steps) {
-            const uint32_t x = key_tile(kc0 + (kLo ? t : t >> 1)), slot = x % kSlots;
-            if (t == 0 || (kLo && t == 1)) ok = warp_wait(bars.full[slot], (x / kSlots) & 1, p.status);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t b = op_desc + slot * (kOpBytes >> 4), a0 = q_desc + (kLo ? 0 : i) * (kOpBytes >> 4);
-            if (elect_one()) {
+            if (more) {
 #pragma unroll
               for (uint32_t part = 0; part < (kLo ? 2u : 1u); ++part)
 #pragma unroll
                 for (uint32_t kk = 0; kk < 8; ++kk)
-                  umma_f16_ss(sc, a0 + (kLo ? 1 - part : 0) * (kOpBytes >> 4) + 16 * kk, b + 16 * kk, kIdesc, part || kk);
+                  umma_f16_ss(sc, a0 + (kLo ? 1 - part : 0) * (kOpBytes >> 4) + 16 * kk, bk + 16 * kk, kIdesc, part || kk);
               umma_commit(smem_addr(&bars.sfull[i]));
-              if (kLo || i == 1) umma_commit(smem_addr(&bars.empty[slot]));
+              if (last) umma_commit(k_bar - smem_addr(&bars.full[0]) + smem_addr(&bars.empty[0]));
               if (t + 1 == n_steps) umma_commit(smem_addr(&bars.qempty));
             }
-            __syncwarp();
+          }
+          __syncwarp();
+          if (pv) {
+            if (i) p_parity[1] ^= 1;
+            else p_parity[0] ^= 1;
+            if (last) two_on(v_slot, v_phase);
+          }
+          if (more && last) {
+            if (first_key) k_slot = 1, first_key = false;   // K0 K1 V0 K2 ..
+            else two_on(k_slot, k_phase);
           }
         }
         ++oc[0];
         if (n_steps > 1) ++oc[1];
-        kc0 += n;
         ++item;
       }
       // every MMA has completed before TMEM is freed
@@ -614,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         if (!raw_ready(0, j) || !slot_free(x)) return false;
         // row = key 64 h + 16 cw + 8 u + kr, chunk 4 g + kq
         uint8_t *kd = smem + kOffOp + (x % kSlots) * kOpBytes + kSbo * (2 * cw) + 16 * kr + kLbo * kq;
-#pragma unroll 1
+#pragma unroll 2
         for (int hu = 0; hu < 4; ++hu) {
           const int h = hu >> 1, u = hu & 1;
           const uint8_t *src = raw_of(0, j) + 4 * h * kHalfBytes;
@@ -639,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         const uint32_t x = value_tile(j);
         if (!raw_ready(1, j) || !slot_free(x)) return false;
         uint8_t *vd = smem + kOffOp + (x % kSlots) * kOpBytes + kLbo * (2 * cw) + 16 * r + 4 * c;
-#pragma unroll 1
+#pragma unroll 2
         for (int hu = 0; hu < 4; ++hu) {
           const int h = hu >> 1, u = hu & 1;
           const uint8_t *src = raw_of(1, j) + 4 * h * kHalfBytes;
@@ -768,10 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           const float sub = m == -INFINITY ? kPShift : kPShift - m;
           const float2 scl2 = make_float2(scl, scl), sub2 = make_float2(sub, sub);
           // 32 scores to P in their own columns: 16 of hi, 16 of lo
-#pragma unroll 1
-          for (uint32_t q = 0; q < 4; ++q) {
-            tmem_ld32(s_col + 32 * q, va);
-            tmem_ld_wait32(va);
+          auto probs = [&](uint32_t q, const uint32_t (&va)[32]) {
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
@@ -787,6 +797,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             }
             tmem_st16(s_col + 32 * q, hi);
             if (kLo) tmem_st16(s_col + 32 * q + 16, lo);
+          };
+          tmem_ld32(s_col, va);
+          if (kLo) {
+#pragma unroll 1
+            for (uint32_t q = 0; q < 4; ++q) {
+              tmem_ld_wait32(va);
+              probs(q, va);
+              if (q < 3) tmem_ld32(s_col + 32 * q + 32, va);
+            }
+          } else {      // the next scores on their way
+            uint32_t vb[32];
+#pragma unroll 1
+            for (uint32_t q = 0; q < 4; q += 2) {
+              tmem_ld_wait32(va);
+              tmem_ld32(s_col + 32 * q + 32, vb);
+              probs(q, va);
+              tmem_ld_wait32(vb);
+              if (q == 0) tmem_ld32(s_col + 64, va);
+              probs(q + 1, vb);
+            }
           }
           tmem_st_wait();
           tc_fence_before();
