@@ -138,6 +138,14 @@ struct Piece {
   uint32_t t0, t1, n;            // key tiles t0 .. t1 - 1 of n; t1 = 0 ends the range
   Kv4Seq s;
   uint32_t c0, c1;               // the ranges that share the piece
+  uint32_t tok0, rem0;           // the row tile's first row as token and head of the group
+  // token and head of the tile's row r: r + rem0 < 272, so 2^16 / group, rounded
+  // up, divides exactly
+  __device__ __forceinline__ void place(uint32_t r, uint32_t group, uint32_t inv, uint32_t *tok, uint32_t *hd) const {
+    const uint32_t x = r + rem0, y = x * inv >> 16;
+    *tok = tok0 + y;
+    *hd = x - y * group;
+  }
 };
 
 // Walks the pieces of a range.  A piece of n key tiles is n + kPieceCost units
@@ -248,7 +256,7 @@ struct Walk {
 // [1, 2)) to fit binary16's range, in place, each lane its own chunks.
 template <class T>
 __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
-                                             uint32_t share) {
+                                             uint32_t inv, uint32_t share) {
   constexpr bool kLo = sizeof(T) == 4, kCopy = __is_same(T, __half);
   constexpr uint32_t MR = kLo ? 128 : 256, kShares = kConvWarps + kQWarps;
   const uint32_t lane = threadIdx.x & 31, kr = lane & 7, kq = lane >> 3, n_rows = pc.s.nq * p.group;
@@ -256,8 +264,9 @@ __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece
   const T *q = static_cast<const T *>(p.q) + pc.s.q0 * p.q_stride + static_cast<size_t>(pc.head) * p.group * kKv4Head + 8 * kq;
 #pragma unroll 1
   for (uint32_t g = share; g < MR / 8; g += kShares) {
-    const uint32_t row = row0 + 8 * g + kr, tok = row / p.group, hd = row - tok * p.group;
-    const bool is = row < n_rows;       // zeros behind the last row
+    uint32_t tok, hd;
+    pc.place(8 * g + kr, p.group, inv, &tok, &hd);
+    const bool is = row0 + 8 * g + kr < n_rows;       // zeros behind the last row
     const T *src = is ? q + tok * p.q_stride + hd * kKv4Head : static_cast<const T *>(p.q);
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
@@ -440,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     auto key_tile = [](uint32_t j) { return kLo ? (j < 2 ? j : 2 * j - 1) : 2 * j; };
     auto value_tile = [](uint32_t j) { return kLo ? 2 * j + 2 : 2 * j + 1; };
     bool ok = true;
+    const uint32_t inv = 65536u / p.group + 1;
     // The range's next piece, for every warp but the loading one.
     uint32_t pieces = 0;
     Piece pc;
@@ -554,6 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         const uint64_t last = walk.first + pc.n;
         pc.c0 = static_cast<uint32_t>(((walk.first + 1) * G - 1) / W);
         pc.c1 = static_cast<uint32_t>((last * G - 1) / W);
+        pc.tok0 = pc.rt * MR / p.group;
+        pc.rem0 = pc.rt * MR - pc.tok0 * p.group;
         if (lane == 0) {
           s_piece[piece_slot] = pc;
           mbar_arrive(smem_addr(&bars.nfull[piece_slot]));
@@ -595,8 +607,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // -------------------------------------------------------- query rows
       uint32_t item = 0;
       while (ok && next_piece()) {
+        // the rows on their way to L2 while the last piece's are in their place:
+        // a lane a row and 128 bytes
+        for (uint32_t x = 32 * (warp - kQ0) + lane; x < MR * (kLo ? 4u : 2u); x += 32 * kQWarps) {
+          const uint32_t r = x / (kLo ? 4u : 2u), part = x % (kLo ? 4u : 2u);
+          uint32_t tok, hd;
+          pc.place(r, p.group, inv, &tok, &hd);
+          if (pc.rt * MR + r < pc.s.nq * p.group)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                reinterpret_cast<const uint8_t *>(static_cast<const T *>(p.q) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.q_stride +
+                                                  (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head) + 128 * part));
+        }
         ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
-        if (ok) load_queries<T>(p, pc, smem + kOffQ, s_scl, warp - kQ0);
+        if (ok) load_queries<T>(p, pc, smem + kOffQ, s_scl, inv, warp - kQ0);
         if (ok && lane == 0) mbar_arrive(smem_addr(&bars.qfull));
         ++item;
       }
@@ -684,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           if (ok && t == 0) {
             ok = item == 0 || warp_wait(bars.qempty, (item - 1) & 1, p.status);
             if (!ok) break;
-            load_queries<T>(p, pc, smem + kOffQ, s_scl, kQWarps + cw);
+            load_queries<T>(p, pc, smem + kOffQ, s_scl, inv, kQWarps + cw);
             if (lane == 0) mbar_arrive(smem_addr(&bars.qfull));
             ++item;
             if (!kLo) ok = values(kc);
@@ -708,7 +731,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       while (ok && next_piece()) {
         const uint32_t n = pc.t1 - pc.t0, n_steps = steps(n), trow = kLo ? row : 128 * i + row;
         const uint32_t grow = pc.rt * MR + trow, n_rows = pc.s.nq * p.group;
-        const uint32_t tok = grow / p.group;
+        uint32_t tok, hd;
+        pc.place(trow, p.group, inv, &tok, &hd);
         // keys that the row sees; a row behind the last is for no use
         const int64_t pos1 = static_cast<int64_t>(pc.s.len) - pc.s.nq + tok + 1;
         const uint32_t limit = grow >= n_rows ? pc.s.len : pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
@@ -846,11 +870,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
         }
         const bool whole = pc.t0 == 0 && pc.t1 == pc.n;
         const bool blind = limit == 0 || grow >= n_rows;
-        const float inv = whole ? 1.f / L : 1.f;
+        const float share = whole ? 1.f / L : 1.f;
         if (whole && !blind && !(M == -INFINITY && L == 0.f) && !(L > 0.f && L < INFINITY && fabsf(M) < INFINITY))
           atomicOr(p.status, ZDEV_ERR_NUMERICAL);
         T *orow = static_cast<T *>(p.out) + (pc.s.q0 + static_cast<uint64_t>(tok)) * p.out_stride +
-                  (static_cast<size_t>(pc.head) * p.group + grow % p.group) * kKv4Head;
+                  (static_cast<size_t>(pc.head) * p.group + hd) * kKv4Head;
         const bool none = M == -INFINITY && L == 0.f;
         float *part = p.part + (2ull * blockIdx.x + (pc.t0 == 0 ? 1 : 0)) * kPartFloats;
         // 32 dims at a time: f32 rows share the row's dims between the streams' warps
@@ -872,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           if (q + 1 < q1) tmem_ld32(o_col + (kLo ? 0 : 128 * i) + 32 * (q + 1), v);
           if (whole) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : o[x] * inv;
+            for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : o[x] * share;
             if (!blind) put32(orow + 32 * q, o, sectors);
           } else {
 #pragma unroll
