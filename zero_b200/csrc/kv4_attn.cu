@@ -483,7 +483,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
         L = 0.f;
         O = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t k0 = c0; k0 <= c1; k0 += 32) {
-          const uint32_t k = k0 + mc;
+          const uint32_t k = k0 + mc, n = min(32u, c1 - k0 + 1);
+          auto sums_of = [&](uint32_t j) {
+            return __ldcg(reinterpret_cast<const float4 *>(p.part + (2ull * (k0 + j) + (k0 + j == c0 ? 1 : 0)) * kPartFloats +
+                                                           mr * kKv4Head + 4 * mc));
+          };
+          // the first sums come with the states: most pieces are cut in few
+          constexpr uint32_t kFirst = 4;
+          float4 first[kFirst];
+#pragma unroll
+          for (uint32_t j = 0; j < kFirst; ++j) first[j] = j < n ? sums_of(j) : make_float4(0.f, 0.f, 0.f, 0.f);
           float2 st = make_float2(-INFINITY, 0.f);
           if (k <= c1)
             st = __ldcg(reinterpret_cast<const float2 *>(p.part + (2ull * k + (k == c0 ? 1 : 0)) * kPartFloats +
@@ -494,16 +503,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
           const float keep = weight(M, nm), w = weight(st.x, nm);
           L *= keep;
           O.x *= keep, O.y *= keep, O.z *= keep, O.w *= keep;
-          const uint32_t n = min(32u, c1 - k0 + 1);
-#pragma unroll 8
-          for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t kj = k0 + j;
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(
-                p.part + (2ull * kj + (kj == c0 ? 1 : 0)) * kPartFloats + mr * kKv4Head + 4 * mc));
+          auto add = [&](uint32_t j, const float4 x) {
             const float wj = __shfl_sync(0xffffffffu, w, j);
             L += __shfl_sync(0xffffffffu, st.y, j) * wj;
             O.x += x.x * wj, O.y += x.y * wj, O.z += x.z * wj, O.w += x.w * wj;
-          }
+          };
+#pragma unroll
+          for (uint32_t j = 0; j < kFirst; ++j)
+            if (j < n) add(j, first[j]);
+#pragma unroll 8
+          for (uint32_t j = kFirst; j < n; ++j) add(j, sums_of(j));
           M = nm;
         }
         whole = true;
