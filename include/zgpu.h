@@ -302,7 +302,7 @@ typedef struct zgpu_kv4_work zgpu_kv4_work;
 zgpu_status zgpu_kv4_create(zgpu_ctx *ctx, uint32_t n_blocks, uint32_t block_tokens, uint32_t n_layers,
                             uint32_t n_kv_heads, uint32_t head_dim, zgpu_kv4 **out);
 void zgpu_kv4_destroy(zgpu_kv4 *kv);
-/* Scratch of the attention (about 44 MB): one serves one call at a time.
+/* Scratch of the attention (about 42 MB): one serves one call at a time.
  * Calls that may overlap on the GPU (two streams, two graphs replayed side by
  * side) need one each, and after ZGPU_ERR_DEVICE_TIMEOUT it has to be made
  * again. */
@@ -336,7 +336,9 @@ zgpu_status zgpu_kv4_plan_device(zgpu_kv4 *kv, uint32_t n_seq, uint32_t table_wi
  * order: their lengths become 0, their table entries ZGPU_KV4_NONE,
  * d_state[0] grows, d_state[1..3] become 0, 0 and the blocks returned.  A
  * table with a block outside the pool, or more blocks than the pool has,
- * changes nothing but d_state[1] = 2. */
+ * changes nothing but d_state[1] = 2.  Rows may share blocks, but a block comes
+ * back once for every released row that lists it: the caller releases a shared
+ * block with one row only (and clears it from the others' tables first). */
 zgpu_status zgpu_kv4_release_device(zgpu_kv4 *kv, uint32_t n_seq, uint32_t table_width, const uint32_t *d_done,
                                     uint32_t *d_lens, uint32_t *d_table, uint32_t *d_free_list, uint32_t *d_state,
                                     void *stream);

