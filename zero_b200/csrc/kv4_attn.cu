@@ -68,8 +68,16 @@ constexpr uint32_t kPartFloats = kRows * (kKv4Head + 2);   // o, max, sum
 constexpr uint32_t kMergeRow = kKv4Head + 4;     // floats between a warp's rows: its stores hit 32 banks
 constexpr uint32_t kMergeFloats = kRows * (kMergeRow + 2);
 constexpr float kPShift = 15.f;                  // P is held times 2^15
-constexpr uint32_t kMinUnits = kWarps / 2;       // a range is worth a unit for every second warp
-constexpr uint32_t kPieceCost = 16;              // what a piece costs beside its units, in units
+// A range is worth a unit for every second warp.  4, 8, 16, 32 units measured in a
+// graph, 16 heads on 8, f32: one sequence of 1000 keys 7.8, 8.0, 9.2, 10.9 us; four
+// of 500 7.9, 9.2, 8.0, 8.0; 16 of 300 11.5, 11.5, 10.7, 13.1; 16 of 1000 14.8,
+// 14.8, 14.8, 15.8.
+constexpr uint32_t kMinUnits = kWarps / 2;
+// What a piece costs beside its units, in units.  4, 8, 16, 32 measured: 16
+// sequences of 128..2047 keys, 32 heads on 8, 19.4, 19.3, 17.9, 20.1 us; in a graph
+// and 16 heads on 8, four of 500 8.6, 8.4, 7.8, 9.6, 64 of 300 20.8, 20.4, 20.1, 17.0;
+// 131071 keys 45.6 to 45.9 with all four.
+constexpr uint32_t kPieceCost = 16;
 
 // Dynamic shared memory: the warps' rings (and, when a piece is done, the
 // warps' states in their places: two CTAs then fit an SM whatever the number of

