@@ -44,6 +44,7 @@
 //   end in units of 32 keys, each behind kPieceCost units for what a piece
 //   costs by itself (queries, merging), and cut into equal ranges, one per
 //   CTA, so a ragged batch or one long sequence keeps every SM equally busy.  A piece
+//   of at most 512 keys is not cut: the border moves to its nearer end.  One
 //   cut by a range boundary leaves unnormalised partials (max, sum, o) in the
 //   workspace; the CTA that arrives last merges them in range order, so the
 //   result does not depend on which one that is.
@@ -78,6 +79,12 @@ constexpr uint32_t kMinUnits = kWarps / 2;
 // and 16 heads on 8, four of 500 8.6, 8.4, 7.8, 9.6, 64 of 300 20.8, 20.4, 20.1, 17.0;
 // 131071 keys 45.6 to 45.9 with all four.
 constexpr uint32_t kPieceCost = 16;
+// A piece of no more units than this is not cut: joining costs as much as it
+// computes.  None, 12, 16 and 32 units, in a graph, 16 heads on 8, f32: 64 sequences
+// of 300 keys 20.1, 16.4, 16.4, 16.4 us, 64 of 500 22.6, 22.8, 18.5, 18.5, 32 of 400
+// 14.8, 14.8, 10.5, 10.5, four of 1000 10.4, 10.5, 10.5, 15.8; one of 131071 46.2,
+// 46.7, 46.9 (the borders' search).
+constexpr uint32_t kWholeUnits = 2 * kWarps;
 
 // Dynamic shared memory: the warps' rings (and, when a piece is done, the
 // warps' states in their places: two CTAs then fit an SM whatever the number of
@@ -197,17 +204,28 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     pdl_wait();
     return;
   }
-  uint64_t at = div64(W * blockIdx.x, G);
-  const uint64_t end = div64(W * (blockIdx.x + 1), G);
-  uint32_t seq = 0;
+  // the range's borders, one to a lane; a border inside a short piece moves to
+  // the nearer end of it (which moves no border into, or out of, a longer one)
+  uint64_t at, end;
+  uint32_t seq;
   {
-    uint32_t lo = 0, hi = p.n_seq;   // sums[lo] <= at < sums[hi]
+    uint64_t border = div64(W * (blockIdx.x + (lane & 1u)), G);
+    uint32_t lo = 0, hi = p.n_seq;   // sums[lo] <= border < sums[hi]
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (sums[mid] <= at) lo = mid;
+      if (sums[mid] <= border) lo = mid;
       else hi = mid;
     }
-    seq = lo;
+    bool bad = false;
+    const uint32_t all = units_of(kv4_seq(p, lo, &bad).len);
+    if (border < W && all <= kWholeUnits + kPieceCost) {
+      const uint64_t in = border - sums[lo];
+      const uint32_t off = static_cast<uint32_t>(in - div64(in, all) * all);
+      border = 2 * off < all ? border - off : border + (all - off);
+    }
+    at = __shfl_sync(0xffffffffu, border, 0);
+    end = __shfl_sync(0xffffffffu, border, 1);
+    seq = __shfl_sync(0xffffffffu, lo, 0);
   }
   uint32_t it0 = 0;         // units that this warp took before the piece: stage and phase of the ring
   bool dead = false;        // a wait of this warp ran out
