@@ -623,6 +623,23 @@ def test_attention_many_short_pieces_per_cta(ctx, dtype, n_seq, n):
     c["kv"].close()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seed", range(6))
+def test_attention_short_and_long_sequences_in_any_order(ctx, dtype, seed):
+    """Pieces that are cut between CTAs beside ones that are not (512 keys and fewer)."""
+    rng = np.random.default_rng(900 + seed)
+    n = int(rng.integers(5, 90))
+    lens = [int(x) for x in np.where(rng.random(n) < 0.5, rng.integers(1, 514, n), rng.integers(500, 2600, n))]
+    nq = [min(x, int(y)) for x, y in zip(lens, rng.integers(0, 4, n))]
+    c = make(ctx, seed, lens, nq, 4, 2, 16 << (seed % 4))
+    o, q = run_attn(c, dtype)
+    check_attn(c, o, q, dtype)
+    o2, _ = run_attn(c, dtype)
+    assert np.array_equal(o, o2)
+    c["kv"].check()
+    c["kv"].close()
+
+
 @pytest.mark.parametrize("nq", [1, 9, 20])
 def test_attention_of_the_most_sequences(ctx, nq):
     """1024 sequences, the largest table of sums; every 64th is checked."""

@@ -51,7 +51,7 @@
 //
 //   Measured: 32 sequences of 8191..32767 keys, 32 heads on 8, bf16: 142 us (156
 //   with inputs that change; 4.2 TB/s); one of 131071 keys, 16 heads on 8, f16:
-//   45 us; one of 500: 7.4 us in a graph, of which the lengths, the table, the
+//   46 us; one of 500: 7.5 us in a graph, of which the lengths, the table, the
 //   words, the split's bookkeeping and the join are each about a microsecond.
 #include "kv4_rows.cuh"
 
