@@ -602,9 +602,10 @@ def test_calls_leave_the_current_device_and_null_rows_alone(ctx):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n_q,n_kv,nq", [
-    (2, 2, [31, 32, 33]), (6, 2, [10, 11, 12]), (4, 1, [8, 9, 1]), (16, 2, [4, 5, 3]), (16, 1, [2, 3, 0]), (11, 1, [3, 2, 3])])
+    (2, 2, [31, 32, 33]), (6, 2, [10, 11, 12]), (4, 1, [8, 9, 1]), (16, 2, [4, 5, 3]), (16, 1, [2, 3, 0]), (11, 1, [3, 2, 3]),
+    (2, 2, [24, 25, 23]), (4, 1, [6, 7, 5]), (12, 1, [2, 3, 1])])
 def test_attention_around_the_border_of_the_two_kernels(ctx, dtype, n_q, n_kv, nq):
-    """Up to 32 query rows per kv head, and more, in one call and in separate ones."""
+    """Up to 32 query rows per kv head (24 in f32) and more, in one call."""
     c = make(ctx, n_q + n_kv, [nq[0] + 200, nq[1], nq[2] + 999], nq, n_q, n_kv, 32)
     o, q = run_attn(c, dtype)
     check_attn(c, o, q, dtype)

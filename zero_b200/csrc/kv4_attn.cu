@@ -4,8 +4,8 @@
 // own position: row i's queries are its last ones, query t of n at position
 // kv_len - n + t.
 //
-// kv4_rows_kernel: at most 32 query rows per kv head (decode, short
-// continuations); kv4_prompt.cu takes the sequences with more.
+// kv4_rows_kernel: at most 32 query rows per kv head, 24 in f32 (decode,
+// short continuations); kv4_prompt.cu takes the sequences with more.
 // Bound by the cache read, 144 bytes per key and kv head, and close behind it
 // by instruction issue: unpacking 256 values per key and head.
 //
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       if (i < p.n_seq) {
         const Kv4Seq s = kv4_seq(p, i, &bad);
         blind |= s.len < s.nq;
-        if (!p.few_only || s.nq * p.group <= kKv4FewRows)
+        if (!p.few_only || s.nq * p.group <= kv4_few_rows(kLo))
           w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * units_of(s.len);
       }
       uint64_t inc = w;
@@ -621,7 +621,7 @@ cudaError_t kv4_attn_setup() {
 
 cudaError_t launch_kv4_attention(const Kv4AttnParams &p, Kv4Type t, int sm_count, uint32_t *launches, cudaStream_t s) {
   Kv4AttnParams few = p;
-  few.few_only = static_cast<uint64_t>(p.max_q) * p.group > kKv4FewRows;
+  few.few_only = static_cast<uint64_t>(p.max_q) * p.group > kv4_few_rows(t == KV4_F32);
   cudaError_t e = cudaSuccess;
   if (few.few_only) {
     Kv4AttnParams many = p;

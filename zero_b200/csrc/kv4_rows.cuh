@@ -96,14 +96,16 @@ __device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, co
 // Query rows per kv head above which a sequence goes to the prompt kernel
 // (kv4_prompt.cu), whose time hardly depends on the rows of a tile, while
 // kv4_attn.cu's grows with every eighth.  Eight kv heads, group of four, us:
-//                        16 rows      32 rows      48 rows      64 rows
+//                        16 rows      24 rows      32 rows      40 rows
 //                      few  prompt  few  prompt  few  prompt  few  prompt
-//   f32  16 x  4096    51.5  84.4   89.5  85.4  127.6  86.8  166.5  87.3
-//         1 x 65536    49.4  94.6   84.3  95.9  120.0  97.2  155.9  97.5
-//         1 x   700    10.5  24.8   12.5  25.1   12.5  26.2   12.7  26.8
-//   f16  16 x  4096    43.9  97.5   75.6  98.5  107.0  99.0  139.0  99.6
-//        64 x   700    43.3  93.0   75.2  94.8  106.8  95.1  137.8  95.9
-//         1 x 65536    42.6 121.9   70.5 122.9   99.6 123.7  128.9 123.9
-constexpr uint32_t kKv4FewRows = 32;
+//   f32  16 x  4096    51.6  74.9   70.4  74.9   89.1  75.6  107.9  76.6
+//        64 x   700    47.6  71.0   66.0  72.0   84.2  72.4  100.6  74.3
+//         1 x 65536    50.0  89.2   66.2  89.6   84.7  89.1  102.4  90.1
+//         1 x   700    10.5  22.7   10.5  22.7   11.6  22.7   12.5  22.8
+//   f16  16 x  4096    44.1  86.0   60.3  86.4   75.8  87.0   92.1  87.5
+//        64 x   700    43.3  79.1   60.0  78.9   75.9  79.3   90.8  80.2
+//         1 x 65536    43.4 114.6   56.2 113.9   71.5 114.2   85.8 114.5
+//         1 x   700    10.5  24.5   10.5  24.8   11.8  24.8   12.2  24.8
+constexpr uint32_t kv4_few_rows(bool f32) { return f32 ? 24u : 32u; }
 
 }  // namespace zgpu
