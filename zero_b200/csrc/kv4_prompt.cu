@@ -593,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
           ent = entry(t + 1);
           if (lane < 8) s_bad[kc & 7][lane] = bad;
           if (bad) atomicOr(p.status, ZDEV_ERR_BOUNDS);
+          __syncwarp();          // lane 0's arrival on rfull publishes what eight lanes stored
 #pragma unroll 1
           for (uint32_t v = 0; ok && v < 2; ++v) {
             if (kc >= kRawStages) ok = warp_wait(bars.rempty[v][stage], (kc / kRawStages - 1) & 1, p.status);
