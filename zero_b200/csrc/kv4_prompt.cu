@@ -254,6 +254,13 @@ struct Walk {
   }
 };
 
+// The factor of a row's scores, scale log2(e) 2^e.  It is at least the smallest
+// normal number: masked scores are -inf before it is applied, and -inf times 0
+// would be NaN.  A score that the floor makes larger is below 2^-88 all the same.
+__device__ __forceinline__ float score_factor(float scale, int e) {
+  return fmaxf(scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 0x1p-126f);
+}
+
 // One of kConvWarps + kQWarps warps' share of a piece's query rows: binary16
 // (hi and lo for f32) in the operand layout, and each row's factor of the
 // scores.  Eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
@@ -281,7 +288,7 @@ __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece
       cp_async16(at + kSbo * g + 4 * kLbo * k, src + (is ? 32 * k : 0), is ? 16u : 0u);
       if (kLo) cp_async16(at + kOpBytes + kSbo * g + 4 * kLbo * k, src + (is ? 32 * k + 4 : 0), is ? 16u : 0u);
     }
-    if (kCopy && kq == 0) s_scl[8 * g + kr] = p.scale * 1.44269504088896341f;
+    if (kCopy && kq == 0) s_scl[8 * g + kr] = score_factor(p.scale, 0);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!kCopy) {
@@ -319,7 +326,7 @@ __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece
       e = e < -100 ? -100 : e > 110 ? 110 : e;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       if (kq == 0)
-        s_scl[8 * g + kr] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        s_scl[8 * g + kr] = score_factor(p.scale, e);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t hi[4], lo[4];
