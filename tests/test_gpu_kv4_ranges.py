@@ -27,3 +27,58 @@ def test_zero_and_tiny_rows_under_a_tiny_scale(ctx, dtype, nq, scale):
     check_attn(c, o, q, dtype, float(np.float32(scale)))
     c["kv"].check()
     c["kv"].close()
+
+
+def cancelling(rng, n, n_kv, amp):
+    """A query of all magnitudes up to 2 amp and keys [n, n_kv, HD] of whole numbers
+    -8..7 (scale 1, exact in the cache), whose products reach 16 amp while
+    their sum is at most about 1."""
+    q = rng.choice([-1.0, 1.0], HD) * amp * np.exp2(-rng.integers(0, 12, HD)) * (1 + rng.random(HD))
+    q = q.astype(np.float16).astype(np.float64)
+    keys = np.zeros((n, n_kv, HD))
+    for t in range(n):
+        for h in range(n_kv):
+            k = rng.integers(-7, 8, HD).astype(np.float64)
+            k[::32] = -8                     # the group's largest: its scale is 1
+            free = np.arange(HD) % 32 != 0
+            for _ in range(400):             # the step that leaves least
+                s = q @ k
+                if abs(s) < 1:
+                    break
+                up, down = np.where(free & (k < 7), abs(s + q), np.inf), np.where(free & (k > -7), abs(s - q), np.inf)
+                i, j = up.argmin(), down.argmin()
+                if min(up[i], down[j]) < abs(s):
+                    k[i if up[i] < down[j] else j] += 1 if up[i] < down[j] else -1
+                else:
+                    k[rng.choice(np.flatnonzero(free))] = rng.integers(-7, 8)
+            keys[t, h] = k
+    return q, keys
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_scores_of_16_bit_rows_are_summed_as_exactly_as_those_of_f32_rows(ctx, dtype, nq):
+    """The same rows in f32 and in 16 bits.  Beside what the f32 call is off by, a
+    16-bit result is off by its own rounding and by a probability of 11 bits;
+    a sum of scores in fewer than f32's bits would show: the largest product is 2048,
+    and a probability's last place is worth 2^-11 of a score."""
+    rng = np.random.default_rng(6)
+    n, n_kv, block = 16 + nq - 1, 2, 16
+    q1, keys = cancelling(rng, n, n_kv, 128.0)
+    q1 = torch.from_numpy(q1).to(TYPES[dtype][0]).double().numpy()
+    kv = cache(ctx, -(-n // block), block, 1, n_kv)
+    vals = rng.standard_normal((n, n_kv, HD)).astype(np.float32)
+    store(kv, 0, np.arange(n, dtype=np.uint32), keys, vals)
+    c = dict(kv=kv, table=np.arange(-(-n // block), dtype=np.uint32)[None], lens=np.array([n], np.uint32),
+             starts=np.array([0, nq], np.uint32), layer=0, n_q=n_kv, n_kv=n_kv, width=-(-n // block),
+             q=np.broadcast_to(q1, (nq, n_kv, HD)).astype(np.float32).copy(), ks=[keys], vs=[R.values(vals)])
+    assert np.array_equal(R.values(keys), keys)
+    wide, q = run_attn(c, "f32", 1.0)
+    o, _ = run_attn(c, dtype, 1.0)
+    ref, mass, _, _ = R.attention(q, keys, c["vs"][0], 1.0)
+    half = torch.finfo(TYPES[dtype][0]).eps / 2
+    tol = 2 * np.abs(wide - ref).max() + 2.0 ** -11 * mass + half * np.abs(ref) + 2.0 ** -21
+    err = np.abs(o - ref)
+    assert (err <= tol).all(), float((err / tol).max())
+    kv.check()
+    kv.close()

@@ -23,15 +23,13 @@
 //   so neither half leaves binary16's range; P is held times 2^15, which
 //   keeps probabilities down to 2^-39 of the row's largest.
 //
-//   Keys stay integers: a masked nibble is a subnormal binary16, n 2^-24 (16
-//   times that at bits 4..7, which the query's other half carries as 1 / 16),
-//   so a value pair costs one logical operation.  Each group of 32 dims has
-//   its own sum, sum_g d_g (sum_j q_j n_j - 8 sum_j q_j), scaled in f32.  The
-//   matrix unit aligns a subnormal's products by its exponent, not by its
-//   leading bit, so their sum keeps some 17 bits: enough for 16-bit rows.  For
-//   f32 rows the words become the normal numbers n - 8 and 16 (n - 8), exact,
-//   with one more operation a pair (error 3e-7 of the result's norm, against
-//   1.7e-6 with the integers).
+//   Keys enter as the whole numbers n - 8, exact: a nibble under the exponent of
+//   1024 (bits 0..3) or of 64 (bits 4..7), less 1032 or 72.  Each group of 32
+//   dims has its own sum, scaled by d_g in f32.  The masked nibble itself would be a
+//   subnormal, n 2^-24, for one operation less a pair, but the matrix unit
+//   aligns a subnormal's products by its exponent, not by its leading bit, so
+//   that their sum keeps some 17 bits: an f16 result whose products reach 2048
+//   was 4e-3 off, and is 3e-4 off with these.
 //   Values are made binary16 by the bits' place: under a fixed exponent a
 //   nibble is a constant plus n, and (16 + n) d - 24 d is one exact fma since
 //   24 d is exact; for 256 + n an add takes the constant off first.
@@ -141,8 +139,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   __shared__ __align__(8) uint64_t bars[kWarps * kStages];
   __shared__ uint64_t s_scan[kWarps];
   __shared__ uint32_t s_last, s_limit[kRows];
-  __shared__ float s_scl[kRows], s_bias[kRows][4];
-  __shared__ __align__(8) uint32_t s_magic[2];
+  __shared__ float s_scl[kRows];
+  __shared__ __align__(8) uint32_t s_magic[4];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   uint64_t *sums = reinterpret_cast<uint64_t *>(smem + kOffSums);   // work before sequence i, n_seq + 1
   auto state_of = [&](uint32_t w) { return reinterpret_cast<float *>(smem + w * kStages * kUnitBytes); };
@@ -230,6 +228,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
   uint32_t it0 = 0;         // units that this warp took before the piece: stage and phase of the ring
   bool dead = false;        // a wait of this warp ran out
   const Magic mg = magic(smem_addr(s_magic));
+  const KMagic kg = k_magic(smem_addr(s_magic + 2));
 
   while (at < end) {
     while (sums[seq + 1] <= at) ++seq;
@@ -307,29 +306,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-      // 256 times: the pairs that meet 16 n are held / 16, their low halves
-      // still far from binary16's subnormals
+      // 256 times: the low halves stay far from binary16's subnormals
       int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
       e = e < -100 ? -100 : e > 110 ? 110 : e;
-      const float down = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23), down16 = down * 0.0625f;
-      const float4 y = make_float4(x.x * down, x.y * down, x.z * down16, x.w * down16);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23);
+      const float4 y = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
       const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
       const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
       *reinterpret_cast<uint4 *>(smem + kOffQ + 512 * (2 * (lane >> 3) + (lane & 1u)) + 16 * (4 * warp + ((lane & 7u) >> 1))) =
           make_uint4(h2bits(h0), h2bits(__floats2half2_rn(y.x - f0.x, y.y - f0.y)), h2bits(h1),
                      h2bits(__floats2half2_rn(y.z - f1.x, y.w - f1.y)));
-      // - 8 sum q of each group, in the units of the products
-      if (!kLo) {
-        float qsum = (y.x + y.y) + 16.f * (y.z + y.w);
-#pragma unroll
-        for (int off = 1; off < 8; off <<= 1) qsum += __shfl_xor_sync(0xffffffffu, qsum, off);
-        if ((lane & 7u) == 0) s_bias[warp][lane >> 3] = qsum * (-8.f * 0x1p-24f);
-      }
       if (lane == 0) {
         // keys that the row sees: 0 .. limit - 1 (none when its position is negative)
         const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + qtok + 1;
         s_limit[warp] = pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
-        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + (kLo ? 0 : 24) - 8 + e) << 23);
+        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 - 8 + e) << 23);
       }
     }
     __syncthreads();
@@ -338,10 +329,6 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
     uint32_t all_see = limit;       // keys that every row sees need no mask
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, off));
-
-    float bias[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) bias[g] = kLo ? 0.f : s_bias[r][g];
 
     // o[n]: dims 16 n + r (and + 8) of rows 2 c and 2 c + 1; m, l: row r
     float o[8][4], m = -INFINITY;
@@ -376,16 +363,15 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
           const uint32_t w = g == 0 ? kw[u].x : g == 1 ? kw[u].y : g == 2 ? kw[u].z : kw[u].w, w8 = w >> 8;
           const uint32_t dw = g == 0 ? kd[u].x : g == 1 ? kd[u].y : g == 2 ? kd[u].z : kd[u].w;
           float sc[4];
-          uint32_t n[4] = {w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
-          if (kLo) {    // 1024 + n, less 1032; 1024 + 16 n, less 1152
+          // 1024 + n, less 1032; 64 + n, less 72
+          uint32_t n[4] = {(w & 0x000F000Fu) | kg.x1024, (w & 0x00F000F0u) | kg.x64, (w8 & 0x000F000Fu) | kg.x1024,
+                           (w8 & 0x00F000F0u) | kg.x64};
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              n[x] = h2bits(__hsub2(bits2h(n[x] | 0x64006400u), bits2h(x & 1 ? 0x64806480u : 0x64086408u)));
-          }
+          for (int x = 0; x < 4; ++x) n[x] = h2bits(__hsub2(bits2h(n[x]), bits2h(x & 1 ? 0x54805480u : 0x64086408u)));
           mma16816_zero(sc, qa.x, qa.y, qa.z, qa.w, n[0], n[1]);
           mma16816(sc, qb.x, qb.y, qb.z, qb.w, n[2], n[3]);
           float2 t = make_float2(sc[0], sc[1]);
-          t = add2_rn(t, kLo ? make_float2(sc[2], sc[3]) : make_float2(bias[g], bias[g]));
+          if (kLo) t = add2_rn(t, make_float2(sc[2], sc[3]));
           v[u] = fma2_rn(t, __half22float2(bits2h(dw)), v[u]);
         }
       }

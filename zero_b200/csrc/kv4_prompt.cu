@@ -74,9 +74,6 @@ struct Bars {
 };
 
 // K's four nibble pairs of a word (bits 0, 4, 8, 12 of each half) as (n - 8) d.
-struct KMagic {
-  uint32_t x1024, x64;
-};
 __device__ __forceinline__ void k_values(uint32_t w, __half2 d, const KMagic &g, uint32_t (&v)[4]) {
   const uint32_t w8 = w >> 8;
   const __half2 m1032 = __half2half2(__ushort_as_half(0xE408)), m72 = __half2half2(__ushort_as_half(0xD480));
@@ -643,9 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
       // --------------------------------------- keys and values to binary16
       const uint32_t cw = warp - kConv0, r = lane >> 2, c = lane & 3, kr = lane & 7, kq = lane >> 3;
       const Magic mg = magic(smem_addr(s_magic));
-      KMagic kg;
-      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_addr(s_magic + 2)), "r"(0x64006400u), "r"(0x54005400u) : "memory");
-      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(kg.x1024), "=r"(kg.x64) : "r"(smem_addr(s_magic + 2)) : "memory");
+      const KMagic kg = k_magic(smem_addr(s_magic + 2));
       // operand tile x may be written once the MMAs that read tile x - 3 are done
       auto slot_free = [&](uint32_t x) { return x < kSlots || warp_wait(bars.empty[x % kSlots], (x / kSlots - 1) & 1, p.status); };
       auto hand_over = [&](uint32_t x) {

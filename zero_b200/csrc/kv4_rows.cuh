@@ -83,6 +83,16 @@ __device__ __forceinline__ Magic magic(uint32_t saddr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(g.x16), "=r"(g.x256) : "r"(saddr) : "memory");
   return g;
 }
+// Likewise those of 1024 and 64, for K.
+struct KMagic {
+  uint32_t x1024, x64;
+};
+__device__ __forceinline__ KMagic k_magic(uint32_t saddr) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(saddr), "r"(0x64006400u), "r"(0x54005400u) : "memory");
+  KMagic g;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(g.x1024), "=r"(g.x64) : "r"(saddr) : "memory");
+  return g;
+}
 // The four V nibbles of both halves of w as (n - 8) d, exactly.
 __device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, const Magic &g, uint32_t (&v)[4]) {
   const uint32_t x = __byte_perm(w, 0u, 0x2301u);
