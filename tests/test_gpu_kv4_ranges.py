@@ -82,3 +82,19 @@ def test_scores_of_16_bit_rows_are_summed_as_exactly_as_those_of_f32_rows(ctx, d
     assert (err <= tol).all(), float((err / tol).max())
     kv.check()
     kv.close()
+
+
+@pytest.mark.parametrize("dtype,gain,scale", [
+    ("f32", 4e37, 2.2e-39), ("f32", 3e36, 2.9e-38), ("f32", 1e-33, 8.8e31), ("f32", 1e-37, 8.8e35), ("f32", 1e-40, 3.3e38),
+    ("bf16", 4e37, 2.2e-39), ("bf16", 3e36, 2.9e-38), ("bf16", 1e-33, 8.8e31), ("bf16", 1e-37, 8.8e35), ("bf16", 1e-40, 3.3e38),
+    ("f16", 1e4, 8.8e-6), ("f16", 3e-7, 3e5), ("f16", 30.0, 0.09), ("bf16", 30.0, 0.09), ("bf16", 1e4, 1e-3)])
+@pytest.mark.parametrize("lens,nq", [([300, 41], [1, 3]), ([300, 141], [160, 141])])
+def test_rows_at_the_ends_of_their_types(ctx, dtype, gain, scale, lens, nq):
+    """Rows of the largest and of subnormal values in both kernels, and sharp
+    scores of 16-bit rows."""
+    c = make(ctx, 50, lens, nq, 4, 2, 16, qgain=gain)
+    o, q = run_attn(c, dtype, scale)
+    assert np.isfinite(q).all() and q.any()
+    check_attn(c, o, q, dtype, float(np.float32(scale)))
+    c["kv"].check()
+    c["kv"].close()

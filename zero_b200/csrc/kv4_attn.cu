@@ -19,8 +19,8 @@
 //   taken transposed, V^T P^T: the scores' fragment is P^T's as it stands, the
 //   values are the sixteen rows, and the result takes half the registers.  For
 //   16-bit rows P is one binary16 value, 11 bits.  A query
-//   row is scaled by a power of two first (its largest value in [256, 512)),
-//   so neither half leaves binary16's range; P is held times 2^15, which
+//   row is scaled by a power of two first (its largest value in [256, 512); a row
+//   below 2^-119 by 2^127), so neither half leaves binary16's range; P is held times 2^15, which
 //   keeps probabilities down to 2^-39 of the row's largest.
 //
 //   Keys enter as the whole numbers n - 8, exact: a nibble under the exponent of
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       for (int off = 1; off < 32; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
       // 256 times: the low halves stay far from binary16's subnormals
       int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-      e = e < -100 ? -100 : e > 110 ? 110 : e;
+      e = e < -119 ? -119 : e > 127 ? 127 : e;
       const float down = __uint_as_float(static_cast<uint32_t>(127 + 8 - e) << 23);
       const float4 y = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
       const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
         // keys that the row sees: 0 .. limit - 1 (none when its position is negative)
         const int64_t pos1 = static_cast<int64_t>(s.len) - s.nq + qtok + 1;
         s_limit[warp] = pos1 > 0 ? static_cast<uint32_t>(pos1) : 0u;
-        s_scl[warp] = p.scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 - 8 + e) << 23);
+        s_scl[warp] = score_factor(p.scale, e - 8);
       }
     }
     __syncthreads();

@@ -251,13 +251,6 @@ struct Walk {
   }
 };
 
-// The factor of a row's scores, scale log2(e) 2^e.  It is at least the smallest
-// normal number: masked scores are -inf before it is applied, and -inf times 0
-// would be NaN.  A score that the floor makes larger is below 2^-88 all the same.
-__device__ __forceinline__ float score_factor(float scale, int e) {
-  return fmaxf(scale * 1.44269504088896341f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 0x1p-126f);
-}
-
 // One of kConvWarps + kQWarps warps' share of a piece's query rows: binary16
 // (hi and lo for f32) in the operand layout, and each row's factor of the
 // scores.  Eight rows at a time, lane (kr, kq) taking chunks kq, kq + 4, kq + 8,
@@ -265,7 +258,8 @@ __device__ __forceinline__ float score_factor(float scale, int e) {
 // contiguous bytes.  All of a warp's rows are on their way at once, copied to
 // where they end up (an f32 chunk's two halves to its hi and its lo place);
 // then f32 and bf16 rows are scaled by a power of two (the largest value in
-// [1, 2)) to fit binary16's range, in place, each lane its own chunks.
+// [2, 4); subnormal rows by 2^127) to fit binary16's range, in place, each lane
+// its own chunks.
 template <class T>
 __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece &pc, uint8_t *q_op, float *s_scl,
                                              uint32_t inv, uint32_t share) {
@@ -320,10 +314,10 @@ __device__ __forceinline__ void load_queries(const Kv4AttnParams &p, const Piece
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
       int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-      e = e < -100 ? -100 : e > 110 ? 110 : e;
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      e = e < -126 ? -126 : e > 127 ? 127 : e;
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 1 - e) << 23);
       if (kq == 0)
-        s_scl[8 * g + kr] = score_factor(p.scale, e);
+        s_scl[8 * g + kr] = score_factor(p.scale, e - 1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t hi[4], lo[4];

@@ -48,6 +48,17 @@ __device__ __forceinline__ void put4(__nv_bfloat16 *p, float4 v) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
 }
 
+// The factor of a row's scores, scale log2(e) 2^e with e in -252..252, applied
+// in two halves: 2^e alone may lie outside the normal numbers.  It is at
+// least the smallest normal number: the prompt kernel's masked scores are -inf
+// before it is applied, and -inf times 0 would be NaN.  A score that the floor
+// makes larger is below 2^-88 all the same.
+__device__ __forceinline__ float score_factor(float scale, int e) {
+  const int a = e >> 1, b = e - a;
+  const float half = scale * __uint_as_float(static_cast<uint32_t>(127 + a) << 23) * 1.44269504088896341f;
+  return fmaxf(half * __uint_as_float(static_cast<uint32_t>(127 + b) << 23), 0x1p-126f);
+}
+
 // One sequence as the call gives it, with lengths that cannot lead outside
 // the buffers; *bad says that they would have.
 struct Kv4Seq {
