@@ -21,7 +21,6 @@ enum : uint32_t {
   ZDEV_ERR_LM_NONFINITE = 1u << 2,
   ZDEV_ERR_LM_PADDING = 1u << 3,
   ZDEV_ERR_BOUNDS = 1u << 4,      // a token / position outside the cache
-  ZDEV_ERR_POOL = 1u << 5,        // paged cache: a plan or release that was refused
 };
 
 // The status block is kStatusWords uint32: word 0 holds the ZDEV_ERR_* bits;

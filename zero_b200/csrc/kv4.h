@@ -60,6 +60,10 @@ __host__ __device__ inline uint32_t kv4_v_nibbles(uint32_t v) {
   return ((v >> 6) & 15u) | ((v >> 2) & 15u) << 4 | ((v >> 10) & 15u) << 8 | ((v >> 14) | (v & 3u) << 2) << 12;
 }
 
+// A bit of the cache's status word beside those of common.cuh: a plan or
+// release that was refused.
+enum : uint32_t { ZDEV_ERR_POOL = 1u << 5 };
+
 // Element types of rows given to append / gather / attention.
 enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2 };
 
