@@ -105,7 +105,7 @@ struct Kv4AttnParams {
   float scale;
   float *part;                // partial slots of the launch's CTAs
   uint32_t *counters;         // zero between calls
-  uint32_t few_only;          // kv4_attn.cu: sequences of more rows go to kv4_prompt.cu
+  uint32_t few_rows;          // sequences of more rows per kv head go to kv4_prompt.cu
   uint32_t *status;
 };
 // Bytes of the partials and the number of counters a workspace needs.

@@ -4,8 +4,8 @@
 // own position: row i's queries are its last ones, query t of n at position
 // kv_len - n + t.
 //
-// kv4_rows_kernel: at most 32 query rows per kv head, 24 in f32 (decode,
-// short continuations); kv4_prompt.cu takes the sequences with more.
+// kv4_rows_kernel: few query rows per kv head (decode, short continuations;
+// kv4_few_rows below); kv4_prompt.cu takes the sequences with more.
 // Bound by the cache read, 144 bytes per key and kv head, and close behind it
 // by instruction issue: unpacking 256 values per key and head.
 //
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       if (i < p.n_seq) {
         const Kv4Seq s = kv4_seq(p, i, &bad);
         blind |= s.len < s.nq;
-        if (!p.few_only || s.nq * p.group <= kv4_few_rows(kLo))
+        if (s.nq * p.group <= p.few_rows)
           w = static_cast<uint64_t>((s.nq * p.group + kRows - 1) / kRows) * p.n_kv * units_of(s.len);
       }
       uint64_t inc = w;
@@ -559,9 +559,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
 }
 
 template <class T>
-cudaError_t launch_rows(const Kv4AttnParams &p, int sm_count, cudaStream_t s) {
+cudaError_t launch_rows(const Kv4AttnParams &p, bool behind, int sm_count, cudaStream_t s) {
   const uint32_t smem = kOffSums + (p.n_seq + 1) * 8;
-  if (!p.few_only) {
+  if (!behind) {
     kv4_rows_kernel<T><<<sm_count * kCtasPerSm, 32 * kWarps, smem, s>>>(p);
     return cudaGetLastError();
   }
@@ -586,6 +586,36 @@ cudaError_t rows_setup() {
                               kOffSums + (kKv4MaxSeqs + 1) * 8);
 }
 
+// Query rows per kv head above which a sequence goes to the prompt kernel
+// (kv4_prompt.cu).  That one's time hardly depends on the rows of a tile, but it
+// starts slowly and joins long sequences in one CTA per kv head; this one's
+// grows by a pass over the cache with every eighth row.  So the border falls with
+// what a pass costs: the keys that the call can read, sequences x kv heads x
+// (table row + 512, a piece's own cost).  us, few rows / prompt kernel, in a graph:
+//                               rows  16          32          48          64          96
+//   f32  1 x   700, 8 kv heads     8.8/20.7    9.8/21.2   10.5/21.9   11.0/22.2   12.0/23.4
+//        1 x  8000, 8             15.0/41.4   19.3/40.6   23.2/41.6   27.8/42.1   35.7/44.1
+//       64 x   700, 1             13.9/26.3   17.9/26.6   23.4/27.3   27.1/27.7   36.4/28.7
+//       16 x   700, 8             17.8/31.8   27.2/32.1   36.3/32.3   44.1/33.0   62.3/33.9
+//        1 x 65536, 8             46.1/85.2   79.3/86.2  113.2/87.5  147.2/88.6  214.8/89.8
+//       16 x  4096, 8             47.4/71.7   84.0/72.6  120.9/74.2  158.6/74.8  231.2/76.3
+//       64 x   700, 8             44.4/69.4   79.5/70.0  114.5/71.9  149.7/73.2  220.9/79.9
+//   f16  1 x   700, 8              9.0/23.3    9.8/23.7   10.8/24.0   10.8/24.6   12.0/25.4
+//        1 x  8000, 8             14.6/57.6   18.2/59.3   21.7/59.9   25.9/60.0   33.5/61.1
+//       64 x   700, 1             13.2/30.1   17.6/30.4   22.5/30.9   26.4/31.2   35.3/32.0
+//       16 x   700, 8             17.6/34.2   26.6/34.5   35.3/34.9   42.7/35.3   60.3/36.1
+//        1 x 65536, 8             43.2/109     73.4/109    104/110     135/110     196/112
+//       16 x  4096, 8             44.7/85.6   78.7/85.9    112/85.7    147/86.5    214/87.1
+//       64 x   700, 8             42.6/76.3   76.7/77.1    110/77.9    144/78.5    210/79.6
+// Groups of 1, 4 and 8 measured alike.  The lengths themselves are on the
+// device: a table wider than its sequences, or idle rows, count as keys and
+// lower the border, to no less than 24 and 32, which is right for large calls.
+uint32_t kv4_few_rows(const Kv4AttnParams &p, bool f32) {
+  const uint64_t keys = static_cast<uint64_t>(p.n_seq) * p.n_kv * ((static_cast<uint64_t>(p.table_width) << p.bt_log2) + 512);
+  const uint64_t rows = (f32 ? 6400000u : 7500000u) / keys, least = f32 ? 24 : 32;
+  return static_cast<uint32_t>(rows < least ? least : rows > 96 ? 96 : rows);
+}
+
 size_t rows_part_floats(int sm_count) { return static_cast<size_t>(sm_count) * kCtasPerSm * 2 * kPartFloats; }
 
 }  // namespace
@@ -607,19 +637,20 @@ cudaError_t kv4_attn_setup() {
 
 cudaError_t launch_kv4_attention(const Kv4AttnParams &p, Kv4Type t, int sm_count, uint32_t *launches, cudaStream_t s) {
   Kv4AttnParams few = p;
-  few.few_only = static_cast<uint64_t>(p.max_q) * p.group > kv4_few_rows(t == KV4_F32);
+  few.few_rows = kv4_few_rows(p, t == KV4_F32);
+  const bool both = static_cast<uint64_t>(p.max_q) * p.group > few.few_rows;
   cudaError_t e = cudaSuccess;
-  if (few.few_only) {
-    Kv4AttnParams many = p;
+  if (both) {
+    Kv4AttnParams many = few;
     many.part = p.part + rows_part_floats(sm_count);
     many.counters = p.counters + static_cast<uint32_t>(sm_count) * kCtasPerSm;
     e = launch_kv4_prompt(many, t, sm_count, s);
     if (e != cudaSuccess) return e;
     if (launches) ++*launches;
   }
-  if (t == KV4_F32) e = launch_rows<float>(few, sm_count, s);
-  else if (t == KV4_F16) e = launch_rows<__half>(few, sm_count, s);
-  else e = launch_rows<__nv_bfloat16>(few, sm_count, s);
+  if (t == KV4_F32) e = launch_rows<float>(few, both, sm_count, s);
+  else if (t == KV4_F16) e = launch_rows<__half>(few, both, sm_count, s);
+  else e = launch_rows<__nv_bfloat16>(few, both, sm_count, s);
   if (e == cudaSuccess && launches) ++*launches;
   return e;
 }

@@ -1,8 +1,8 @@
 // kv4_prompt.cu — attention of prompts and prompt chunks over the paged 4-bit
 // KV cache, on tcgen05.
 //
-// The same formula as kv4_attn.cu for sequences with more than 32 query rows
-// per kv head (24 in f32).  Bound by the tensor cores (4 * 128 flops per query head and
+// The same formula as kv4_attn.cu for sequences with many query rows per kv head
+// (kv4_few_rows there).  Bound by the tensor cores (4 * 128 flops per query head and
 // key, twice that for f32 rows) and, as closely, by the exponentials: 128 x
 // 128 scores are 1024 cycles of either.
 //
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
     bool bad = false;                     // recorded by the few-rows kernel
     const Kv4Seq s = kv4_seq(p, i, &bad);
     lens[i] = s.len;
-    nqs[i] = s.nq * p.group > kv4_few_rows(kLo) ? s.nq : 0u;
+    nqs[i] = s.nq * p.group > p.few_rows ? s.nq : 0u;
     q0s[i] = s.q0;
   }
   tc_fence_before();

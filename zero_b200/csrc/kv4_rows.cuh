@@ -114,19 +114,4 @@ __device__ __forceinline__ void v_values(uint32_t w, __half2 d, __half2 m24d, co
   v[3] = h2bits(__hfma2(bits2h((x & 0x03C003C0u) | g.x16), d, m24d));
 }
 
-// Query rows per kv head above which a sequence goes to the prompt kernel
-// (kv4_prompt.cu), whose time hardly depends on the rows of a tile, while
-// kv4_attn.cu's grows with every eighth.  Eight kv heads, group of four, us:
-//                        16 rows      24 rows      32 rows      40 rows
-//                      few  prompt  few  prompt  few  prompt  few  prompt
-//   f32  16 x  4096    51.6  74.9   70.4  74.9   89.1  75.6  107.9  76.6
-//        64 x   700    47.6  71.0   66.0  72.0   84.2  72.4  100.6  74.3
-//         1 x 65536    50.0  89.2   66.2  89.6   84.7  89.1  102.4  90.1
-//         1 x   700    10.5  22.7   10.5  22.7   11.6  22.7   12.5  22.8
-//   f16  16 x  4096    44.1  86.0   60.3  86.4   75.8  87.0   92.1  87.5
-//        64 x   700    43.3  79.1   60.0  78.9   75.9  79.3   90.8  80.2
-//         1 x 65536    43.4 114.6   56.2 113.9   71.5 114.2   85.8 114.5
-//         1 x   700    10.5  24.5   10.5  24.8   11.8  24.8   12.2  24.8
-constexpr uint32_t kv4_few_rows(bool f32) { return f32 ? 24u : 32u; }
-
 }  // namespace zgpu
