@@ -68,3 +68,30 @@ def test_small_chunks_by_the_prompt_kernel(ctx, dtype):
     assert np.array_equal(o, o2)
     c["kv"].check()
     c["kv"].close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,nq", [(6, 2, [40, 1]), (192, 96, [17, 2]), (96, 96, [33, 1])])
+def test_rows_on_16_byte_boundaries(ctx, dtype, n_q, n_kv, nq):
+    """q and out 16 bytes behind a wider boundary, at strides that are odd multiples of
+    16 bytes, through both kernels; the gaps stay as they are."""
+    td, zd = TYPES[dtype]
+    unit = 16 // td.itemsize
+    c = make(ctx, n_q, [nq[0] + 300, nq[1] + 40], nq, n_q, n_kv, 16)
+    T, width = sum(nq), n_q * 128 + unit
+    q = torch.zeros(T * width + unit, dtype=td, device="cuda")
+    q[unit:].view(T, width)[:, :n_q * 128] = dev(c["q"]).to(td).flatten(1)
+    host = q[unit:].view(T, width)[:, :n_q * 128].reshape(T, n_q, 128).double().cpu().numpy()
+    for x in (c, widen(c, 16)):
+        out = torch.full_like(q, 3.0)
+        st, ln, tb = dev(x["starts"]), dev(x["lens"]), dev(x["table"])
+        torch.cuda.synchronize()
+        c["kv"].attention_device(0, 2, T, max(nq), n_q, q.data_ptr() + 16, out.data_ptr() + 16, st.data_ptr(),
+                                 ln.data_ptr(), tb.data_ptr(), x["width"], dtype=zd, q_stride=width, out_stride=width,
+                                 stream=1)
+        torch.cuda.synchronize()
+        o = out.double().cpu().numpy()
+        assert (o[:unit] == 3).all() and (o[unit:].reshape(T, width)[:, n_q * 128:] == 3).all()
+        check_attn(c, o[unit:].reshape(T, width)[:, :n_q * 128].reshape(T, n_q, 128), host, dtype)
+    c["kv"].check()
+    c["kv"].close()

@@ -37,3 +37,72 @@ def test_append_refuses_every_magnitude_above_its_limit(ctx, dtype):
     store(kv, 0, np.zeros(1, np.uint32), x, -x, dtype)
     kv.check()
     kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n_kv", [1, 7, 96, 1000])
+def test_append_and_gather_on_16_byte_boundaries_and_many_heads(ctx, dtype, n_kv):
+    """Rows that start 16 bytes behind a wider boundary, at strides that are odd
+    multiples of 16 bytes."""
+    td, zd = TYPES[dtype]
+    unit = 16 // td.itemsize
+    n, wide = 21, n_kv * HD + unit
+    rng = np.random.default_rng(n_kv)
+    kv = cache(ctx, 3, 16, 1, n_kv)
+    k, v = (torch.from_numpy(rng.standard_normal(n * wide + unit).astype(np.float32)).to(td).cuda() for _ in range(2))
+    gk, gv = (torch.full_like(k, 5.0) for _ in range(2))
+    slots = rng.permutation(48)[:n].astype(np.uint32)
+    ds = dev(slots)
+    at = unit * td.itemsize
+    kv.append_device(0, n, k.data_ptr() + at, v.data_ptr() + at, ds.data_ptr(), dtype=zd, k_stride=wide, v_stride=wide, stream=1)
+    kv.gather_device(0, n, ds.data_ptr(), gk.data_ptr() + at, gv.data_ptr() + at, dtype=zd, k_stride=wide, v_stride=wide, stream=1)
+    torch.cuda.synchronize()
+    for x, g in ((k, gk), (v, gv)):
+        rows, got = (a[unit:].reshape(n, wide).double().cpu().numpy() for a in (x, g))
+        want = torch.from_numpy(R.values(rows[:, :n_kv * HD].reshape(n, n_kv, HD))).to(td).double().numpy()
+        assert np.array_equal(got[:, :n_kv * HD].reshape(n, n_kv, HD), want)
+        assert (got[:, n_kv * HD:] == 5).all() and (g[:unit] == 5).all()
+    kv.check()
+    kv.close()
+
+
+@pytest.mark.parametrize("n,width,block,share", [(1024, 40, 16, 0.5), (1024, 3, 128, 1.0), (37, 5000, 16, 0.3), (1000, 9, 32, 0.0)])
+def test_release_of_many_rows(ctx, n, width, block, share):
+    rng = np.random.default_rng(n + width)
+    lens = rng.integers(0, width * block + 1, n).astype(np.uint32)
+    lens[:2] = [0, width * block]
+    held = -(-lens.astype(np.int64) // block)
+    n_blocks = int(held.sum()) + 7
+    order = rng.permutation(n_blocks).astype(np.uint32)
+    table = np.full((n, width), NONE, np.uint32)
+    at = 0
+    for i in range(n):
+        table[i, :held[i]] = order[at:at + held[i]]
+        at += held[i]
+    free = np.full(n_blocks, NONE, np.uint32)
+    free[:7] = order[at:]
+    done = (rng.random(n) < share).astype(np.uint32) * rng.integers(1, 1 << 32, n).astype(np.uint32)
+    kv = cache(ctx, n_blocks, block, 1, 1)
+
+    def go(table, lens):
+        b = [dev(a) for a in (done, lens, table, free, np.array([7, 1, 2, 3], np.uint32))]
+        kv.release_device(n, width, *[x.data_ptr() for x in b], stream=1)
+        torch.cuda.synchronize()
+        return [u32(x) for x in b[1:]]
+
+    ln, tab, fl, st = go(table, lens)
+    back = np.concatenate([table[i, :held[i]] for i in range(n) if done[i]] + [np.zeros(0, np.uint32)])
+    assert np.array_equal(ln, np.where(done != 0, 0, lens)) and list(st) == [7 + len(back), 0, 0, len(back)]
+    assert np.array_equal(fl[:7 + len(back)], np.concatenate([free[:7], back])) and (fl[7 + len(back):] == NONE).all()
+    assert np.array_equal(tab, np.where(done[:, None] != 0, NONE, table))
+    kv.check()
+    if done.any():              # one bad block in the last row that ends refuses the whole call
+        i = int(np.flatnonzero((done != 0) & (held > 0))[-1])
+        broken = table.copy()
+        broken[i, held[i] - 1] = n_blocks
+        ln, tab, fl, st = go(broken, lens)
+        assert np.array_equal(ln, lens) and np.array_equal(tab, broken) and np.array_equal(fl, free) and list(st) == [7, 2, 2, 3]
+        with pytest.raises(zb.ZgpuError) as e:
+            kv.check()
+        assert e.value.status == 13
+    kv.close()
