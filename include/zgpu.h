@@ -363,7 +363,8 @@ zgpu_status zgpu_kv4_gather_device(zgpu_kv4 *kv, uint32_t layer, uint32_t n_toke
  * h / (n_q_heads / n_kv_heads); max_q is at least every sequence's number of
  * queries.  Sums and softmax are held in f32; with ZGPU_F32 rows the products
  * keep 22 bits of q and of the probabilities, with 16-bit rows at least
- * binary16's 11.  out must not overlap q.  A sequence with more than max_q
+ * binary16's 11.  Rows may be of any finite magnitude, and scores (scale * q k)
+ * as large as 10^8.  out must not overlap q.  A sequence with more than max_q
  * queries, or whose rows are not within n_rows, gets no output; keys whose
  * block is not in the pool are left out; both are recorded. */
 zgpu_status zgpu_kv4_attention_device(zgpu_kv4 *kv, zgpu_kv4_work *work, uint32_t layer, uint32_t n_seq,

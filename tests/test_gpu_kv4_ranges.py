@@ -98,3 +98,34 @@ def test_rows_at_the_ends_of_their_types(ctx, dtype, gain, scale, lens, nq):
     check_attn(c, o, q, dtype, float(np.float32(scale)))
     c["kv"].check()
     c["kv"].close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 3, 140])
+@pytest.mark.parametrize("size", [1e5, 3e6, 4e7, 1e8])
+def test_scores_far_apart(ctx, dtype, nq, size):
+    """Scores up to 10^8: a row is the value of its largest score, to that value's
+    rounding, where the next score is clearly smaller, and finite anyway.  With
+    16-bit rows the probability, 1 up to a power of two that need not be whole, is
+    one binary16 value over an f32 sum: 2^-11 on top."""
+    c = make(ctx, 60, [700, nq + 90], [nq, nq], 4, 2, 16, qgain=30.0)
+    scale = float(np.float32(size / (30 * 40)))         # the largest q k of some hundred keys is about 30 x 40
+    o, q = run_attn(c, dtype, scale)
+    half = torch.finfo(TYPES[dtype][0]).eps / 2
+    clear = 0
+    for i, n in enumerate(c["lens"]):
+        a = int(c["starts"][i])
+        _, _, _, ds = R.attention(q[a:a + nq], c["ks"][i], c["vs"][i], scale)
+        for t in range(nq):
+            see = int(n) - nq + t + 1
+            for h in range(4):
+                s = c["ks"][i][:see, h // 2] @ q[a + t, h] * scale
+                first, second = np.argsort(-s)[:2]
+                row, v = o[a + t, h], c["vs"][i][:see, h // 2]
+                assert np.isfinite(row).all() and (np.abs(row) <= np.abs(v).max(0) * (1 + 2 * half + 2.0 ** -11) + 2.0 ** -20).all()
+                if s[first] - s[second] > 2 * ds[t, h] + 40:      # the others weigh less than e^-40
+                    clear += 1
+                    assert (np.abs(row - v[first]) <= (half + 2.0 ** -20 + (2.0 ** -11 if dtype != "f32" else 0)) * np.abs(v[first]) + 2.0 ** -30).all()
+    assert clear > nq or size > 1e7
+    c["kv"].check()
+    c["kv"].close()

@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, off));
 
-    // o[n]: dims 16 n + r (and + 8) of rows 2 c and 2 c + 1; m, l: row r
+    // o[n]: dims 16 n + r (and + 8) of rows 2 c and 2 c + 1; m (the exponent that P is
+    // held relative to), l: row r
     float o[8][4], m = -INFINITY;
     float2 l = make_float2(0.f, 0.f);
 #pragma unroll
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
           v[u] = fma2_rn(t, __half22float2(bits2h(dw)), v[u]);
         }
       }
-      float mx = m;
+      float mx = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = mul2_rn(v[u], make_float2(scl, scl));
       if (key0 + kUnit > all_see || (bad_now | bad_before)) {
@@ -396,6 +397,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       for (int u = 0; u < 4; ++u) mx = fmaxf(mx, fmaxf(v[u].x, v[u].y));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // P is 2^(v - m) with m the largest score less kPShift, rounded up: rounded
+      // otherwise, P could pass binary16's range for scores from 2^24
+      mx = fmaxf(m, __fadd_ru(mx, -kPShift));
       const float ms = mx == -INFINITY ? 0.f : mx;
       if (__any_sync(0xffffffffu, mx > m)) {
         const float a = ex2(m - ms);
@@ -411,7 +415,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm) kv4_rows_kernel(const
       uint32_t ph[4], pl[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float2 e = add2_rn(v[u], make_float2(kPShift - ms, kPShift - ms)), pr = make_float2(ex2(e.x), ex2(e.y));
+        const float2 e = add2_rn(v[u], make_float2(-ms, -ms)), pr = make_float2(ex2(e.x), ex2(e.y));
         l = add2_rn(l, pr);
         const __half2 hi = __floats2half2_rn(pr.x, pr.y);
         ph[u] = h2bits(hi);

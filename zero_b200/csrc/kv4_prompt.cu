@@ -789,7 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
             for (int x = 0; x < 32; x += 2)
               mx4[(x >> 1) & 3] = fmaxf(fmaxf(mx4[(x >> 1) & 3], __uint_as_float(va[x])), __uint_as_float(va[x + 1]));
           }
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scl;
+          // P is 2^(score - m) with m the largest score less kPShift, rounded up:
+          // rounded otherwise, P could pass binary16's range for scores from 2^24
+          const float mx = __fmaf_ru(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), scl, -kPShift);
           if (t < 2) {
             m = mx;
           } else if (__any_sync(0xffffffffu, mx > m + kLazy)) {
@@ -807,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Kv4AttnPa
               tmem_st32(o_col + 128 * i + 32 * q, va);
             }
           }
-          const float sub = m == -INFINITY ? kPShift : kPShift - m;
+          const float sub = m == -INFINITY ? 0.f : -m;
           const float2 scl2 = make_float2(scl, scl), sub2 = make_float2(sub, sub);
           // 32 scores to P in their own columns: 16 of hi, 16 of lo
           auto probs = [&](uint32_t q, const uint32_t (&va)[32]) {
