@@ -282,7 +282,9 @@ zgpu_status zgpu_gqa_attention_decode_noalloc(zgpu_ctx *ctx, zgpu_kv *kv, uint32
  * number = block * block_tokens + offset, ZGPU_KV4_NONE for none.  A block
  * table row lists a sequence's blocks in order.  Lengths, tables, slots and
  * row starts are arrays of uint32_t in device memory, so that a step's sizes
- * need not be known to the host.
+ * need not be known to the host.  Rows may share full blocks (a common
+ * prefix); a row that gets new tokens has its last, partly filled block to
+ * itself, or two rows' tokens go to one slot.
  *
  * Calls.  The _device entry points launch on `stream` (NULL: the context's
  * stream; cudaStreamLegacy names the default stream) without synchronising,
@@ -366,7 +368,8 @@ zgpu_status zgpu_kv4_gather_device(zgpu_kv4 *kv, uint32_t layer, uint32_t n_toke
  * binary16's 11.  Rows may be of any finite magnitude, and scores (scale * q k)
  * as large as 10^8.  out must not overlap q.  A sequence with more than max_q
  * queries, or whose rows are not within n_rows, gets no output; keys whose
- * block is not in the pool are left out; both are recorded. */
+ * block is not in the pool are left out; both are recorded.  With n_rows or
+ * max_q 0 the call does nothing. */
 zgpu_status zgpu_kv4_attention_device(zgpu_kv4 *kv, zgpu_kv4_work *work, uint32_t layer, uint32_t n_seq,
                                       uint32_t n_rows, uint32_t max_q, uint32_t n_q_heads, const void *d_q,
                                       uint64_t q_stride, void *d_out, uint64_t out_stride, uint32_t dtype,

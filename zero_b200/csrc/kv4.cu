@@ -146,8 +146,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const Kv4PlanPar
 
 // ---------------------------------------------------------------- release
 // One CTA: pushes the blocks of the rows marked done onto the free list in
-// row order (bound by latency).  A row whose table or the list cannot be right (a block outside
-// the pool, more blocks than the pool has) changes nothing at all.
+// row order.  A row whose table or the list cannot be right (a block outside
+// the pool, more blocks than the pool has) changes nothing at all.  16 rows of
+// up to 128 blocks take 4.2 us in a graph, bound by latency; beyond some
+// thousand blocks the one CTA's accesses bound it: 1024 rows of 64 blocks 40 us,
+// of 1056 blocks 284 us.
 constexpr uint32_t kReleaseThreads = kKv4MaxSeqs;
 
 __global__ void __launch_bounds__(kReleaseThreads) kv4_release_kernel(const Kv4ReleaseParams p) {
@@ -347,7 +350,9 @@ constexpr uint32_t kRowWarps = 8;
 // lane 4 g + c of a half its dims 32 g + 8 c + 0..7.
 // Bound by instruction issue, close above the reads of the rows: 16384 tokens
 // of 8 kv heads in f32 take 37.6 us (134 MB in, 19 MB out, 4.1 TB/s), 203
-// instructions a warp and row pair at 72 % issue.  Four values of both rows a
+// instructions a warp and row pair at 72 % issue (33.3 us in a graph).  16-bit
+// rows are coarser: of normal values a tie sends 34 % of the warps in f16 and 49 %
+// in bf16 into the exact rounding, 47.0 and 50.3 us in a graph (67 MB in).  Four values of both rows a
 // lane took 47 us: the group's maximum, scale and sign cost as much for four
 // values as for eight.  Four CTAs fit an SM at 57 registers; bounds for five and
 // six, at the price of the values on their way, measured 40 and 49 us.
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
 
 // A warp per (token, kv head), four values of both rows a lane, so that a store
 // is 512 contiguous bytes.  Bound by the writes: 16384 tokens of 8 kv heads to f32
-// take 29.5 us (134 MB out, 19 MB in, 5.2 TB/s).
+// take 29.5 us (134 MB out, 19 MB in, 5.2 TB/s), to f16 or bf16 25.5 us.
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_gather_kernel(const Kv4RowsParams p) {
   // the number of warps is a multiple of n_kv: a warp keeps its head

@@ -10,8 +10,9 @@
 // kernels feed the tensor cores the cache's values without a rounding.
 //
 // Why 8 bits of scale: binary16's own 11 would make q * d a 14-bit product
-// that the 16-bit operands round, and the rounding of d costs nothing, since
-// q is chosen against the d that is stored.
+// that the 16-bit operands round, and the rounding of d costs next to nothing,
+// since q is chosen against the d that is stored: normal rows are 8.596 % off
+// (root mean square) with 8 bits of d, with 11 and with 24, and 8.602 % with 6.
 //
 // Storage is by tiles of 16 tokens of one kv head, 2304 contiguous bytes (one
 // bulk copy, or one for each half): K nibbles (1024), K scales (128), V nibbles

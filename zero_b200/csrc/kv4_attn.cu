@@ -18,7 +18,9 @@
 //   kernel has to spare; both halves of a score land in one thread.  P V is
 //   taken transposed, V^T P^T: the scores' fragment is P^T's as it stands, the
 //   values are the sixteen rows, and the result takes half the registers.  For
-//   16-bit rows P is one binary16 value, 11 bits.  A query
+//   16-bit rows P is one binary16 value, 11 bits, as many as an f16 result has: the
+//   second half would double P V's products (an f16 result is 2.5e-4 off with one
+//   half, 2.0e-4 by its own rounding; a bf16 result 1.7e-3 either way).  A query
 //   row is scaled by a power of two first (its largest value in [256, 512); a row
 //   below 2^-119 by 2^127), so neither half leaves binary16's range; P is held times 2^15, which
 //   keeps probabilities down to 2^-39 of the row's largest.
@@ -47,10 +49,12 @@
 //   workspace; the CTA that arrives last merges them in range order, so the
 //   result does not depend on which one that is.
 //
-//   Measured: 32 sequences of 8191..32767 keys, 32 heads on 8, bf16: 142 us (156
-//   with inputs that change; 4.2 TB/s); one of 131071 keys, 16 heads on 8, f16:
-//   46 us; one of 500: 7.5 us in a graph, of which the lengths, the table, the
-//   words, the split's bookkeeping and the join are each about a microsecond.
+//   Measured: 32 sequences of 8191..32767 keys, 32 heads on 8, bf16: 164 us with
+//   inputs that change (4.0 TB/s; 148 in a graph, f32 164); one of 131071 keys, 16
+//   heads on 8, f16: 48.7 us (46.8 in a graph); one of 500: 7.8 us in a graph, of
+//   which the lengths, the table, the words, the split's bookkeeping and the join
+//   are each about a microsecond.  128 registers; the 16-bit forms spill 84 bytes
+//   a thread, f32 16.
 #include "kv4_rows.cuh"
 
 namespace zgpu {

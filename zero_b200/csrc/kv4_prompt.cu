@@ -34,8 +34,8 @@
 //
 // The work is cut into equal ranges of key tiles as in kv4_attn.cu; pieces cut
 // by a range boundary leave partials that the last CTA to arrive joins.
-// Measured: eight prompts of 1021..2048 tokens, 32 heads on 8, f16: 210 us (224
-// with inputs that change), 36 % of the tensor cores' time; a prompt of 2048 in
+// Measured: eight prompts of 1021..2048 tokens, 32 heads on 8, f16: 225 us with
+// inputs that change (207 in a graph, 36 % of the tensor cores' time); a prompt of 2048 in
 // f32, 16 heads on 8: 59 us.  The MMA warp, the conversion and the streams'
 // chains take about as long as each other (3000 to 4400 cycles a key tile).
 // Every wait is bounded; on an expired one each role stops, the MMA thread
